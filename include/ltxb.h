@@ -91,8 +91,9 @@ const char* ltxb_last_error(void);
 const char* ltxb_version(void);
 
 /* Read (and, if clear != 0, reset) the device status word of the current
- * device: LTXB_OK, or LTXB_ETIMEOUT when a kernel's bounded mbarrier/peer
- * wait expired; *site (optional) receives the failing wait's site code.
+ * device: LTXB_OK, LTXB_ETIMEOUT when a kernel's bounded mbarrier/peer wait
+ * expired, or LTXB_EINVAL when a kernel met a bad page number, length or row
+ * range of a 4-bit cache; *site (optional) receives the site code.
  * Synchronises the device. */
 int ltxb_device_status(int clear, uint32_t* site);
 
@@ -479,6 +480,91 @@ int ltxb_denoise_run(const ltxb_core* core, const ltxb_weights* const* blocks, i
  * ltxb_stats_workspace_bytes() bytes of device memory, 16-byte aligned. */
 uint64_t ltxb_stats_workspace_bytes(void);
 int ltxb_stats(const float* v, uint64_t n, float* out, void* workspace, uint64_t workspace_bytes, void* stream);
+
+/* ---- 4-bit K/V cache: writing, reading, attention ------------------------
+ * K/V rows of 128-dim heads kept in 4 bits, so that a sequence (a clip that
+ * is denoised part by part, a prompt model's tokens) keeps 136 .. 160 bytes
+ * per token and head instead of 512. No counterpart in the reference, which
+ * keeps no K/V between calls; the group quantisation follows its grouped-128
+ * weights.
+ *
+ * Values: the 128 values of a token's head fall into groups of `group` = 32,
+ * 64 or 128; each group stores zero = min and scale = bf16((max - min) / 15)
+ * as bf16, and per value code = round((x - zero) / scale) in 0 .. 15 (ties to
+ * even, 0 where scale is 0). A code stands for zero + scale * code. A group
+ * that holds a NaN or an infinity reads back as NaN.
+ *
+ * Pages: LTXB_KV4_PAGE tokens of every head. `pages` is
+ * [n_pages][kv_heads][ltxb_kv4_block_bytes(group)] bytes, 16-byte aligned;
+ * token t of sequence b lies in page page_table[b * max_pages + t / 64] at
+ * t % 64 (page_table NULL: page b * max_pages + t / 64). The bytes of a
+ * block, with nibble n the low (even n) or high half of byte n / 2:
+ *   [0, 4096)     K codes: dim d of token t is nibble
+ *                 ((d / 8) % 4) * 32 + (d / 32) * 8 + d % 8 from byte 64 t
+ *   [4096, 8192)  V codes: nibble (d / 32) * 4 + d % 4 from byte
+ *                 512 (t / 8) + 64 ((d / 4) % 8) + 16 ((t % 8) / 2) + 8 (t % 2)
+ *   then K and V pairs, each [64 tokens][128 / group] of (scale, zero) bf16.
+ *
+ * Rows of a call: sequence b owns rows [row_start[b], row_start[b + 1]) of the
+ * call's tensors (row_start: batch + 1 device int32 in order; rows outside
+ * every range are left alone), or rows / batch rows each with row_start NULL.
+ * They are its LAST tokens: seq_lens[b] counts them already, and row i of n
+ * is token seq_lens[b] - n + i (a negative one does not exist: nothing is
+ * written or read for it, and causally it attends to nothing). So appending
+ * a step's K/V and attending with its queries take the same arguments.
+ *
+ * Lengths, page numbers and row ranges are read on the device (calls can be
+ * captured into a CUDA graph and replayed with other lengths). A page number
+ * outside [0, n_pages), a length outside [0, capacity] or a range outside
+ * [0, rows] is not followed: its tokens are neither written, read nor
+ * attended to (a length is held at the capacity), and ltxb_device_status
+ * reports LTXB_EINVAL with the site LTXB_SITE_KV4_*. Two sequences may share
+ * pages for reading; a page that two rows of one append write to at the same
+ * place holds a mixture of the two. */
+#define LTXB_KV4_PAGE 64
+#define LTXB_SITE_KV4_PAGE 0x401
+#define LTXB_SITE_KV4_LEN 0x402
+#define LTXB_SITE_KV4_ROWS 0x403
+typedef struct {
+  void* pages;
+  const int32_t* page_table; /* [batch, max_pages] device, or NULL            */
+  const int32_t* seq_lens;   /* [batch] device: tokens held, this call's included */
+  int32_t n_pages;
+  int32_t kv_heads;
+  int32_t group;             /* 32, 64 or 128 values per (scale, zero)        */
+  int32_t batch;             /* sequences                                     */
+  int32_t max_pages;         /* pages of a sequence; capacity 64 * max_pages  */
+  int32_t max_len;           /* a bound on seq_lens that the host knows (0: the capacity) */
+} ltxb_kv4_cache;
+
+/* Bytes of one (page, head) block: 8192 + 512 * 128 / group; 0 for another group. */
+uint64_t ltxb_kv4_block_bytes(int group);
+
+/* Quantise k, v [rows, kv_heads, 128] bf16 (row strides ldk, ldv elements, so
+ * that slices of a fused projection can be passed) into the cache. k and v
+ * 16-byte aligned, strides multiples of 8. */
+int ltxb_kv4_append(const ltxb_kv4_cache* cache, const int32_t* row_start, const void* k, int64_t ldk, const void* v,
+                    int64_t ldv, int rows, void* stream);
+
+/* Read the tokens of the call's rows back: k_out, v_out [rows, kv_heads, 128]
+ * contiguous, bf16 or f32 (zero + scale * code in f32, rounded once). Rows
+ * without a token are left as they were. */
+int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k_out, void* v_out, int out_dtype,
+                  int rows, void* stream);
+
+/* out = softmax(q k^T * scale) v over each sequence's cache: q, out
+ * [rows, H, 128] bf16 (q's row stride ldq elements; out contiguous), query
+ * head h reading K/V head h / (H / kv_heads). causal != 0: a row sees the
+ * tokens up to its own; else all of its sequence's. A row that sees nothing
+ * is zero. `gate` (optional, f32 [rows, H]) multiplies each head's output.
+ * A row that attends to a token with a NaN group is NaN. The codes enter the
+ * products exactly; q is bf16, softmax and sums are f32. `workspace`
+ * (256-byte aligned, ltxb_attention_kv4_workspace_bytes bytes) need not be
+ * cleared; calls that may run at the same time need one each. */
+uint64_t ltxb_attention_kv4_workspace_bytes(const ltxb_kv4_cache* cache, int rows, int H);
+int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, const void* q, int64_t ldq, void* out,
+                       const float* gate, int rows, int H, int causal, float scale, void* workspace,
+                       uint64_t workspace_bytes, void* stream);
 
 /* Size of the scratch ltxb_dq_gemm_noalloc keeps in the library image. */
 #define LTXB_NOALLOC_SCRATCH_BYTES (32u << 20)

@@ -147,6 +147,9 @@ int rope_tables(int kind, const float* pos, int T, int H, double theta, float* c
 // status word of the attention unit (compiled separately, see common.cuh)
 cudaError_t attn_status(uint32_t* v, bool clear);
 
+// first bad index that a 4-bit cache kernel met (its site; kv4_cache.cu), 0 if none
+cudaError_t index_status(uint32_t* v, bool clear);
+
 // ---- elementwise / normalisation kernels ----
 // n = rms(x) * (1 + ada(r_scale)) + ada(r_shift) -> bf16 or f32 [T, D]; tstab has tk rows
 int norm_modulate(const float* x, int T, int D, const float* sst, const float* tstab, const int* tidx, int tk, int r_shift,

@@ -247,8 +247,14 @@ int ltxb_device_status(int clear, uint32_t* site) {
   e = ltxb::attn_status(&va, clear != 0);
   if (e != cudaSuccess) return set_cuda_error(e, "read attention status");
   if (!v) v = va;
-  if (site) *site = v >> 8;
+  uint32_t vi = 0;
+  e = ltxb::index_status(&vi, clear != 0);
+  if (e != cudaSuccess) return set_cuda_error(e, "read index status");
+  if (site) *site = v ? v >> 8 : vi;
   if ((v & 0xFF) == STATUS_TIMEOUT) return set_error(LTXB_ETIMEOUT, "device wait expired at site 0x%x", v >> 8);
+  if (vi)
+    return set_error(LTXB_EINVAL, "a 4-bit cache's %s is out of range (site 0x%x)",
+                     vi == LTXB_SITE_KV4_PAGE ? "page number" : vi == LTXB_SITE_KV4_LEN ? "length" : "row_start", vi);
   return LTXB_OK;
 }
 

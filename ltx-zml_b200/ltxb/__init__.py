@@ -55,7 +55,7 @@ def _load() -> ctypes.CDLL:
     if not LIB_PATH.exists():
         raise ImportError(f"{LIB_PATH} is not built (run `make -C ltx-zml_b200` or __graft_entry__.build())")
     lib = ctypes.CDLL(str(LIB_PATH))
-    vp, i32, u64, f32 = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_float
+    vp, i32, u64, f32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_float, ctypes.c_int64
     sig = {
         "ltxb_init": (i32, [i32]),
         "ltxb_last_error": (ctypes.c_char_p, []),
@@ -119,6 +119,11 @@ def _load() -> ctypes.CDLL:
         "ltxb_attention_split": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, f32, i32, vp, u64, vp]),
         "ltxb_dq_gemm": (i32, [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, u64, vp]),
         "ltxb_gemm_bf16": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
+        "ltxb_kv4_block_bytes": (u64, [i32]),
+        "ltxb_kv4_append": (i32, [vp, vp, vp, i64, vp, i64, i32, vp]),
+        "ltxb_kv4_read": (i32, [vp, vp, vp, vp, i32, i32, vp]),
+        "ltxb_attention_kv4_workspace_bytes": (u64, [vp, i32, i32]),
+        "ltxb_attention_kv4": (i32, [vp, vp, vp, i64, vp, vp, i32, i32, i32, f32, vp, u64, vp]),
         "ltxb_stats_workspace_bytes": (u64, []),
         "ltxb_stats": (i32, [vp, u64, vp, vp, u64, vp]),
     }
@@ -146,7 +151,8 @@ def version() -> str:
 
 
 def device_status(clear: bool = True) -> int:
-    """LTXB_OK or LTXB_ETIMEOUT (a bounded device wait expired). Syncs the device."""
+    """LTXB_OK, LTXB_ETIMEOUT (a bounded device wait expired) or LTXB_EINVAL (a
+    4-bit cache's page number, length or row range out of range). Syncs the device."""
     site = ctypes.c_uint32(0)
     return lib.ltxb_device_status(int(clear), ctypes.byref(site))
 
@@ -829,6 +835,137 @@ def attention_split(q, k, v, gate=None, splits: int = 0, scale: float | None = N
         workspace = torch.empty(max(int(need), 1), dtype=torch.uint8, device=q.device)
     _check(lib.ltxb_attention_split(_ptr(q), _ptr(k), _ptr(v), _ptr(out), _ptr(gate), Tq, k.shape[0], H,
                                     float(scale), int(splits), _ptr(workspace), workspace.numel(), _stream(stream)))
+    return out
+
+
+# ---------------------------------------------------------------------------
+# 4-bit K/V cache
+# ---------------------------------------------------------------------------
+
+KV4_PAGE = 64
+SITE_KV4_PAGE, SITE_KV4_LEN, SITE_KV4_ROWS = 0x401, 0x402, 0x403
+
+
+class _KV4(ctypes.Structure):
+    _fields_ = [("pages", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p),
+                ("n_pages", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("group", ctypes.c_int32),
+                ("batch", ctypes.c_int32), ("max_pages", ctypes.c_int32), ("max_len", ctypes.c_int32)]
+
+
+def _row_tensor(t, heads: int, name: str, device) -> int:
+    """Row stride of a [rows, heads, 128] bf16 CUDA tensor whose rows are contiguous."""
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != 128:
+        raise LtxbError(EINVAL, f"{name} must be bf16 [rows, {heads}, 128], got {t.dtype} {list(t.shape)}")
+    if t.device != device:
+        raise LtxbError(EINVAL, f"{name} is on {t.device}, the cache on {device}")
+    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != 128):
+        raise LtxbError(EINVAL, f"{name}: a row's heads must be contiguous")
+    # one row has no stride of its own
+    return t.stride(0) if t.shape[0] > 1 else heads * 128
+
+
+def _index_tensor(t, shape, name: str, device) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device or not t.is_contiguous():
+        raise LtxbError(EINVAL, f"{name} must be a contiguous int32 tensor of shape {list(shape)} on {device}")
+    return t.data_ptr()
+
+
+class KV4Cache:
+    """A paged 4-bit K/V cache (ltxb_kv4_cache; format in include/ltxb.h).
+
+    `pages` uint8 [n_pages, kv_heads, block bytes], `page_table` int32
+    [batch, max_pages] or None (sequence b owns pages b * max_pages ..),
+    `seq_lens` int32 [batch]: tokens held, which the caller moves on (the
+    calls read it on the device; the rows of a call are a sequence's last
+    tokens and are counted in it already)."""
+
+    def __init__(self, batch: int, max_len: int, kv_heads: int, group: int = 128, device="cuda"):
+        block = int(lib.ltxb_kv4_block_bytes(int(group)))
+        if not block:
+            raise LtxbError(EINVAL, f"group must be 32, 64 or 128, got {group}")
+        max_pages = -(-max_len // KV4_PAGE)
+        pages = torch.zeros(batch * max_pages, kv_heads, block, dtype=torch.uint8, device=device)
+        self._bind(pages, None, torch.zeros(batch, dtype=torch.int32, device=pages.device), group, max_pages, max_len)
+
+    @classmethod
+    def from_pages(cls, pages, page_table, seq_lens, group: int = 128, max_len: int = 0) -> "KV4Cache":
+        """A cache over the caller's pool of pages. max_len: a bound on the
+        lengths that is known on the host (0: the page table's capacity)."""
+        block = int(lib.ltxb_kv4_block_bytes(int(group)))
+        if not block:
+            raise LtxbError(EINVAL, f"group must be 32, 64 or 128, got {group}")
+        if pages.dtype != torch.uint8 or pages.dim() != 3 or pages.shape[2] != block or not pages.is_contiguous():
+            raise LtxbError(EINVAL, f"pages must be contiguous uint8 [n_pages, kv_heads, {block}]")
+        if page_table.dim() != 2:
+            raise LtxbError(EINVAL, "page_table must be [batch, max_pages]")
+        c = cls.__new__(cls)
+        c._bind(pages, page_table, seq_lens, group, page_table.shape[1], max_len)
+        return c
+
+    def _bind(self, pages, page_table, seq_lens, group, max_pages, max_len):
+        assert pages.is_cuda, "tensors passed to libltxb must be contiguous CUDA tensors"
+        self.pages, self.page_table, self.seq_lens = pages, page_table, seq_lens
+        self.device, self.group = pages.device, group
+        self.batch, self.kv_heads, self.max_pages = seq_lens.shape[0], pages.shape[1], max_pages
+        _index_tensor(seq_lens, (self.batch,), "seq_lens", self.device)
+        _index_tensor(page_table, (self.batch, max_pages), "page_table", self.device)
+        self._c = _KV4(pages.data_ptr(), None if page_table is None else page_table.data_ptr(), seq_lens.data_ptr(),
+                       pages.shape[0], self.kv_heads, group, self.batch, max_pages, int(max_len))
+        self._ref = ctypes.byref(self._c)
+
+    def _call(self, fn, stream, *args) -> None:
+        """The library runs on the current device: make it the cache's."""
+        if torch.cuda.current_device() == self.device.index:
+            _check(fn(self._ref, *args, _stream(stream)))
+        else:
+            with torch.cuda.device(self.device):
+                _check(fn(self._ref, *args, _stream(stream)))
+
+    def append(self, k, v, row_start=None, stream=None) -> None:
+        """Quantise k, v [rows, kv_heads, 128] bf16 (rows may be strided) into the sequences' last tokens."""
+        ldk, ldv = _row_tensor(k, self.kv_heads, "k", self.device), _row_tensor(v, self.kv_heads, "v", self.device)
+        if k.shape[0] != v.shape[0]:
+            raise LtxbError(EINVAL, "k and v have different numbers of rows")
+        rs = _index_tensor(row_start, (self.batch + 1,), "row_start", self.device)
+        self._call(lib.ltxb_kv4_append, stream, rs, k.data_ptr(), ldk, v.data_ptr(), ldv, k.shape[0])
+
+    def read(self, rows: int, row_start=None, dtype=torch.bfloat16, out=None, stream=None):
+        """K and V [rows, kv_heads, 128] of the sequences' last tokens, bf16 or
+        f32. Rows without a token are left as they were (undefined where the
+        outputs are allocated here)."""
+        if dtype not in (torch.bfloat16, torch.float32):
+            raise LtxbError(EINVAL, "read: dtype must be bfloat16 or float32")
+        if out is None:
+            out = tuple(torch.empty(rows, self.kv_heads, 128, dtype=dtype, device=self.device) for _ in range(2))
+        for t in out:
+            if t.dtype != dtype or tuple(t.shape) != (rows, self.kv_heads, 128) or t.device != self.device:
+                raise LtxbError(EINVAL, f"read: outputs must be {dtype} [{rows}, {self.kv_heads}, 128] on {self.device}")
+        rs = _index_tensor(row_start, (self.batch + 1,), "row_start", self.device)
+        self._call(lib.ltxb_kv4_read, stream, rs, _ptr(out[0]), _ptr(out[1]),
+                   DT_F32 if dtype == torch.float32 else DT_BF16, rows)
+        return out
+
+
+def attention_kv4(q, cache: KV4Cache, row_start=None, causal: bool = True, gate=None, scale: float | None = None,
+                  out=None, workspace=None, stream=None) -> torch.Tensor:
+    """softmax(q k^T * scale) v over each sequence's 4-bit cache; q [rows, H,
+    128] bf16 (rows may be strided), H a multiple of the cache's heads, the
+    rows a sequence's last tokens. gate: f32 [rows, H] or None."""
+    rows, H, hd = q.shape
+    ldq = _row_tensor(q, H, "q", cache.device)
+    out = torch.empty(rows, H, hd, dtype=torch.bfloat16, device=q.device) if out is None else out
+    if out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != q.device:
+        raise LtxbError(EINVAL, "out must be bf16 like q")
+    if gate is not None and (gate.dtype != torch.float32 or tuple(gate.shape) != (rows, H) or gate.device != q.device):
+        raise LtxbError(EINVAL, f"gate must be f32 [{rows}, {H}] on {q.device}")
+    rs = _index_tensor(row_start, (cache.batch + 1,), "row_start", cache.device)
+    if workspace is None:
+        need = int(lib.ltxb_attention_kv4_workspace_bytes(cache._ref, rows, H))
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    cache._call(lib.ltxb_attention_kv4, stream, rs, q.data_ptr(), ldq, _ptr(out), _ptr(gate), rows, H, int(causal),
+                1.0 / np.sqrt(hd) if scale is None else float(scale), _ptr(workspace), workspace.numel())
     return out
 
 
