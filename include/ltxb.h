@@ -566,6 +566,20 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
                        const float* gate, int rows, int H, int causal, float scale, void* workspace,
                        uint64_t workspace_bytes, void* stream);
 
+/* out[M, N] (bf16) = A[M, K] (bf16) . dequant(Wq, scales)^T (+ bias[N] bf16,
+ * optional) with 4-bit weights: ltxb_dq_gemm's linear at half the bytes, from
+ * single rows (a token, a timestep's modulation) up. Wq [N, K / 2] bytes, the
+ * even column in a byte's low half; w = (code - 8) * scale, code 0 .. 15,
+ * scales [N, K / group] f32 or bf16, group 32, 64 or 128. K a multiple of
+ * 128, N of 32; all pointers 16-byte aligned. Few rows read the weights once,
+ * with exact products and f32 sums, and need no workspace; more rows expand
+ * them to bf16 into `workspace` (ltxb_dq4_gemm_workspace_bytes: 0, or
+ * N * K * 2) for the tensor-core GEMM. Each call writes what it reads there;
+ * calls that may run at the same time need one each. */
+uint64_t ltxb_dq4_gemm_workspace_bytes(int M, int N, int K);
+int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_dtype, int group, const void* bias,
+                  void* out, int M, int N, int K, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* Size of the scratch ltxb_dq_gemm_noalloc keeps in the library image. */
 #define LTXB_NOALLOC_SCRATCH_BYTES (32u << 20)
 

@@ -22,6 +22,7 @@ is no fallback.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import json
 import pathlib
@@ -119,6 +120,8 @@ def _load() -> ctypes.CDLL:
         "ltxb_attention_split": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, f32, i32, vp, u64, vp]),
         "ltxb_dq_gemm": (i32, [vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, vp, u64, vp]),
         "ltxb_gemm_bf16": (i32, [vp, vp, vp, vp, i32, i32, i32, vp]),
+        "ltxb_dq4_gemm_workspace_bytes": (u64, [i32, i32, i32]),
+        "ltxb_dq4_gemm": (i32, [vp, vp, vp, i32, i32, vp, vp, i32, i32, i32, vp, u64, vp]),
         "ltxb_kv4_block_bytes": (u64, [i32]),
         "ltxb_kv4_append": (i32, [vp, vp, vp, i64, vp, i64, i32, vp]),
         "ltxb_kv4_read": (i32, [vp, vp, vp, vp, i32, i32, vp]),
@@ -203,6 +206,14 @@ def _ptr(t) -> int | None:
         return None
     assert t.is_cuda and t.is_contiguous(), "tensors passed to libltxb must be contiguous CUDA tensors"
     return t.data_ptr()
+
+
+_HERE_NOW = contextlib.nullcontext()
+
+
+def _device(dev):
+    """The library runs on the current device: a context in which that is `dev`."""
+    return _HERE_NOW if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _stream(stream) -> int:
@@ -916,12 +927,8 @@ class KV4Cache:
         self._ref = ctypes.byref(self._c)
 
     def _call(self, fn, stream, *args) -> None:
-        """The library runs on the current device: make it the cache's."""
-        if torch.cuda.current_device() == self.device.index:
+        with _device(self.device):
             _check(fn(self._ref, *args, _stream(stream)))
-        else:
-            with torch.cuda.device(self.device):
-                _check(fn(self._ref, *args, _stream(stream)))
 
     def append(self, k, v, row_start=None, stream=None) -> None:
         """Quantise k, v [rows, kv_heads, 128] bf16 (rows may be strided) into the sequences' last tokens."""
@@ -995,6 +1002,46 @@ def dq_gemm(a, wq, scales, bias=None, fused: bool = True, out=None, workspace=No
         workspace = torch.empty(N * K * 2, dtype=torch.uint8, device=a.device)
     _check(lib.ltxb_dq_gemm(_ptr(a), _ptr(wq), _ptr(scales), sdt, _ptr(bias), _ptr(out), M, N, K, int(fused),
                             _ptr(workspace), 0 if workspace is None else workspace.numel(), _stream(stream)))
+    return out
+
+
+def quantize_g4(w, group: int = 128, scale_dtype=torch.bfloat16):
+    """4-bit weights for dq4_gemm from w [N, K]: (uint8 [N, K / 2], scales [N, K / group])
+    with scale = max|w| / 7 of a group (at least 1e-12, as the int8 quantiser of
+    tools/quantize_block.py:40-59), code = round(w / scale) + 8."""
+    N, K = w.shape
+    if group not in (32, 64, 128) or K % group or scale_dtype not in (torch.bfloat16, torch.float32):
+        raise LtxbError(EINVAL, f"quantize_g4: group {group} of K = {K}, scales {scale_dtype}")
+    g = w.float().view(N, K // group, group)
+    scale = (g.abs().amax(-1) / 7).clamp_min(1e-12).to(scale_dtype)
+    code = (torch.round(g / scale.float()[..., None]).clamp_(-8, 7) + 8).to(torch.uint8).view(N, K)
+    return (code[:, 0::2] | (code[:, 1::2] << 4)).contiguous(), scale.contiguous()
+
+
+def dq4_gemm(a, wq, scales, bias=None, out=None, workspace=None, stream=None) -> torch.Tensor:
+    """a [M, K] bf16 . dequant(wq uint8 [N, K / 2], scales [N, K / group] f32 or
+    bf16)^T (+ bias bf16) -> bf16 [M, N]: the linear with 4-bit weights
+    (quantize_g4), the group being K over the scales' columns."""
+    M, K = a.shape
+    N = wq.shape[0]
+    dev = a.device
+    if (a.dtype != torch.bfloat16 or wq.dtype != torch.uint8 or tuple(wq.shape) != (N, K // 2)
+            or scales.dtype not in (torch.bfloat16, torch.float32) or scales.shape[0] != N or K % scales.shape[1]):
+        raise LtxbError(EINVAL, "dq4_gemm: a bf16 [M, K], wq uint8 [N, K / 2], scales f32 or bf16 [N, K / group]")
+    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,)):
+        raise LtxbError(EINVAL, f"dq4_gemm: bias must be bf16 [{N}]")
+    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if out is None else out
+    if out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
+        raise LtxbError(EINVAL, f"dq4_gemm: out must be bf16 [{M}, {N}]")
+    if any(t is not None and t.device != dev for t in (wq, scales, bias, out, workspace)):
+        raise LtxbError(EINVAL, "dq4_gemm: tensors on different devices")
+    if workspace is None:
+        need = int(lib.ltxb_dq4_gemm_workspace_bytes(M, N, K))
+        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _device(dev):
+        _check(lib.ltxb_dq4_gemm(_ptr(a), _ptr(wq), _ptr(scales), DT_BF16 if scales.dtype == torch.bfloat16 else DT_F32,
+                                 K // scales.shape[1], _ptr(bias), _ptr(out), M, N, K, _ptr(workspace),
+                                 0 if workspace is None else workspace.numel(), _stream(stream)))
     return out
 
 

@@ -118,3 +118,23 @@ def test_no_rows_is_no_work():
     assert ltxb.lib.ltxb_kv4_read(r, None, None, None, ltxb.DT_BF16, 0, None) == ltxb.OK
     assert ltxb.lib.ltxb_attention_kv4(r, None, None, 256, None, None, 0, 2, 1, 0.1, None, 0, None) == ltxb.OK
     assert ltxb.launch_count() == n0
+
+
+def test_bad_4bit_linear_calls_are_refused():
+    import ltxb
+    buf = ctypes.create_string_buffer(1 << 12)
+    at = (ctypes.addressof(buf) + 255) & ~255
+    f, big = ltxb.lib.ltxb_dq4_gemm, 1 << 40
+    n0 = ltxb.launch_count()
+
+    def call(A=at, W=at, S=at, dt=ltxb.DT_F32, group=128, bias=None, out=at, M=1, N=32, K=128, ws=at, wb=big):
+        return f(A, W, S, dt, group, bias, out, M, N, K, ws, wb, None)
+    refused = [call(dt=ltxb.DT_I8), call(group=16), call(group=256), call(M=-1), call(N=0), call(N=48), call(K=64),
+               call(K=0), call(A=at + 2), call(A=None), call(W=at + 8), call(W=None), call(S=at + 4), call(S=None),
+               call(out=at + 2), call(out=None), call(bias=at + 2), call(M=1000, wb=100), call(M=1000, ws=None),
+               call(M=1000, ws=at + 8)]
+    assert refused == [ltxb.EINVAL] * len(refused)
+    assert call(M=0, A=None, W=None) == ltxb.OK
+    assert ltxb.launch_count() == n0
+    assert ltxb.lib.ltxb_dq4_gemm_workspace_bytes(1, 32, 128) == 0
+    assert ltxb.lib.ltxb_dq4_gemm_workspace_bytes(1000, 32, 128) == 32 * 128 * 2
