@@ -515,10 +515,10 @@ int ltxb_stats(const float* v, uint64_t n, float* out, void* workspace, uint64_t
  *
  * Lengths, page numbers and row ranges are read on the device (calls can be
  * captured into a CUDA graph and replayed with other lengths). A page number
- * outside [0, n_pages), a length outside [0, capacity] or a range outside
- * [0, rows] is not followed: its tokens are neither written, read nor
- * attended to (a length is held at the capacity), and ltxb_device_status
- * reports LTXB_EINVAL with the site LTXB_SITE_KV4_*. Two sequences may share
+ * outside [0, n_pages) is not followed: its tokens are neither written nor
+ * read, and a row that attends to one is NaN. A length is held within
+ * [0, capacity], a row range within [0, rows]. ltxb_device_status then reports
+ * LTXB_EINVAL with the site LTXB_SITE_KV4_*. Two sequences may share
  * pages for reading; a page that two rows of one append write to at the same
  * place holds a mixture of the two. */
 #define LTXB_KV4_PAGE 64
@@ -557,10 +557,15 @@ int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k
  * head h reading K/V head h / (H / kv_heads). causal != 0: a row sees the
  * tokens up to its own; else all of its sequence's. A row that sees nothing
  * is zero. `gate` (optional, f32 [rows, H]) multiplies each head's output.
- * A row that attends to a token with a NaN group is NaN. The codes enter the
- * products exactly; q is bf16, softmax and sums are f32. `workspace`
- * (256-byte aligned, ltxb_attention_kv4_workspace_bytes bytes) need not be
- * cleared; calls that may run at the same time need one each. */
+ * A row that attends to a token with a NaN group is NaN. Softmax, sums and
+ * accumulators are f32. With fewer than 64 query rows a sequence and K/V head
+ * (on average: rows * H / kv_heads / batch) the cache is read as it is and its
+ * codes enter the products exactly; with more, K and V are laid out in the
+ * workspace as f16 (one rounding of 2^-12) for the tcgen05 kernel, which takes
+ * 512 bytes per token and head up to the capacity (max_len, if given, is what
+ * it is sized by). `workspace` (256-byte aligned,
+ * ltxb_attention_kv4_workspace_bytes bytes) need not be cleared; calls that
+ * may run at the same time need one each. */
 uint64_t ltxb_attention_kv4_workspace_bytes(const ltxb_kv4_cache* cache, int rows, int H);
 int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, const void* q, int64_t ldq, void* out,
                        const float* gate, int rows, int H, int causal, float scale, void* workspace,

@@ -149,6 +149,8 @@ cudaError_t attn_status(uint32_t* v, bool clear);
 
 // first bad index that a 4-bit cache kernel met (its site; kv4_cache.cu), 0 if none
 cudaError_t index_status(uint32_t* v, bool clear);
+// status word of kv4_attn_tc.cu (a unit of its own, like the attention's)
+cudaError_t kv4_attn_status(uint32_t* v, bool clear);
 
 // ---- elementwise / normalisation kernels ----
 // n = rms(x) * (1 + ada(r_scale)) + ada(r_shift) -> bf16 or f32 [T, D]; tstab has tk rows

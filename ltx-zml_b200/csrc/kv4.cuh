@@ -43,8 +43,12 @@ struct Kv4View {
 // the kernels: a bad one is not followed, and its site is kept in a word of
 // its own (not in g_status: a bad page of one caller must not make other
 // kernels' waits give up).
+#ifdef LTXB_LOCAL_STATUS  // kv4_attn_tc.cu: the operand kernels of the same call have reported
+__device__ __forceinline__ void report_index(uint32_t) {}
+#else
 extern __device__ uint32_t g_index_status;
 __device__ __forceinline__ void report_index(uint32_t site) { atomicCAS(&g_index_status, 0u, site); }
+#endif
 
 // Tokens of sequence b in the cache, in [0, cap].
 __device__ __forceinline__ int kv4_len(const Kv4View& v, int b) {
@@ -98,6 +102,25 @@ __device__ __forceinline__ int kv4_row_seq(const Kv4View& v, int i) {
 __device__ __forceinline__ const uint8_t* kv4_block_at(const Kv4View& v, int page, int head, int bytes) {
   return v.pages + ((size_t)page * v.heads + head) * bytes;
 }
+
+// ---- many-row attention: operands in the workspace (kv4_prep.cu, kv4_attn_tc.cu) ----
+struct Kv4Tc {
+  void* q16;         // f16 [heads][rows * G][128]: row `row * G + g` of a K/V head
+  float* q_scale;    // [heads][rows * G]: softmax scale * log2(e) / the row's power of two
+  void* k16;         // f16 [batch * heads][tokens][128]
+  void* v16;
+  float2* top;       // [batch * heads][chunks]: largest |K|, |V| of 16 pages
+  float2* kv_scale;  // [batch * heads]: 1 / the powers of two of K and V
+  float* o_part;     // [splits][heads][rows * G][128], with splits > 1
+  float* ml_part;    // [splits][heads][rows * G][2]: reference maximum, sum
+  int tokens, chunks, G, splits;
+  float cs;          // softmax scale * log2(e)
+};
+int kv4_prepare(const Kv4View& c, const Kv4Tc& t, const void* q, size_t ldq, int group, cudaStream_t st);
+int kv4_attention_tc(const Kv4View& c, const Kv4Tc& t, const float* gate, void* out, int causal, cudaStream_t st);
+// rows of a query tile pair, and the K/V splits that fill the GPU
+constexpr int KV4_TC_ROWS = 256;
+int kv4_tc_splits(const Kv4View& c, int G);
 
 // host side (kv4_cache.cu): argument checks shared by the entry points
 int kv4_check(const ltxb_kv4_cache* c, const int32_t* row_start, int rows, const char* what, Kv4View* out);

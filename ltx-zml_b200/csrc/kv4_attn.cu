@@ -27,9 +27,9 @@
 // A page's block for one head (8.5 - 10 KB) arrives by one bulk copy into a
 // ring of KA_STAGES, so 4 CTAs keep about 100 KB per SM in flight.
 //
-// A token whose V group is stored as NaN makes its score NaN (every row that
-// attends to it becomes NaN) and is left out of the product, so that rows
-// which do not attend to it stay finite.
+// A token whose V group is stored as NaN, or whose page number is bad, makes
+// its score NaN (every row that attends to it becomes NaN) and is left out of
+// the product, so that rows which do not attend to it stay finite.
 #include <float.h>
 
 #include <atomic>
@@ -315,7 +315,8 @@ __global__ void __launch_bounds__(KA_THREADS, R == 8 ? 4 : 3) kv4_attn_kernel(co
       const uint8_t* blk = ring + st * BLK;
       const int t0 = warp * 16 + g;  // this lane's tokens t0 and t0 + 8 of the page
       const int key0 = at.page * KV4_PAGE + t0, key1 = key0 + 8;
-      const int len = sm.good[st] ? at.len : 0;
+      const int len = at.len;
+      const bool good = sm.good[st] != 0;
       // ---- S^T: 16 tokens x R rows ----
       float s[NT][4];
       {
@@ -370,13 +371,14 @@ __global__ void __launch_bounds__(KA_THREADS, R == 8 ? 4 : 3) kv4_attn_kernel(co
           sv1[x] = bf16_lo(p1);
           zv0[x] = fmaf(8.f, sv0[x], bf16_hi(p0));
           zv1[x] = fmaf(8.f, sv1[x], bf16_hi(p1));
-          // a group that is not finite, or a token behind the last one: out of the product
-          if (key0 >= len || !(fabsf(zv0[x]) < INFINITY)) {
-            bad0 = zv0[x] - zv0[x];  // NaN where the group is not finite
+          // a group that is not finite, a page that was not read, a token behind
+          // the last one (which the mask takes out): not in the product
+          if (key0 >= len || !good || !(fabsf(zv0[x]) < INFINITY)) {
+            bad0 = NAN;
             sv0[x] = zv0[x] = 0.f;
           }
-          if (key1 >= len || !(fabsf(zv1[x]) < INFINITY)) {
-            bad1 = zv1[x] - zv1[x];
+          if (key1 >= len || !good || !(fabsf(zv1[x]) < INFINITY)) {
+            bad1 = NAN;
             sv1[x] = zv1[x] = 0.f;
           }
           svm = fmaxf(svm, fmaxf(sv0[x], sv1[x]));
@@ -634,6 +636,45 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const KaArgs a) {
 // host side
 // ---------------------------------------------------------------------------
 
+// Many rows a sequence and K/V head: the tcgen05 kernel over f16 operands in
+// the workspace. Below this the page kernel above, which reads the cache once
+// per 16 rows, is faster than laying the operands out.
+constexpr int KV4_TC_MIN = 64;
+constexpr uint64_t KV4_TC_BYTES = 24ull << 30;  // and never for operands beyond this
+
+static uint64_t kv4_tc_layout(const Kv4View& c, int G, Kv4Tc* t, void* ws) {
+  uint64_t at = 0;
+  uint8_t* base = static_cast<uint8_t*>(ws);
+  auto take = [&](uint64_t bytes) {
+    uint8_t* p = base ? base + at : nullptr;
+    at += (bytes + 255) & ~uint64_t(255);
+    return p;
+  };
+  const uint64_t qr = (uint64_t)c.heads * c.rows * G, bh = (uint64_t)c.batch * c.heads;
+  t->G = G;
+  t->tokens = (c.cap + 127) / 128 * 128;
+  t->chunks = (t->tokens / KV4_PAGE + 15) / 16;
+  t->splits = kv4_tc_splits(c, G);
+  t->q16 = take(qr * KV4_D * 2);
+  t->q_scale = reinterpret_cast<float*>(take(qr * 4));
+  t->k16 = take(bh * t->tokens * KV4_D * 2);
+  t->v16 = take(bh * t->tokens * KV4_D * 2);
+  t->top = reinterpret_cast<float2*>(take(bh * t->chunks * 8));
+  t->kv_scale = reinterpret_cast<float2*>(take(bh * 8));
+  t->o_part = reinterpret_cast<float*>(take(t->splits > 1 ? t->splits * qr * KV4_D * 4 : 0));
+  t->ml_part = reinterpret_cast<float*>(take(t->splits > 1 ? t->splits * qr * 8 : 0));
+  return at;
+}
+
+// Whether a call takes the tcgen05 path, and its workspace there.
+static bool kv4_use_tc(const Kv4View& c, int G, uint64_t* bytes, Kv4Tc* t) {
+  if ((int64_t)c.rows * G < (int64_t)KV4_TC_MIN * c.batch || c.cap == 0 || c.batch > 65535 || c.heads > 65535) return false;
+  if ((int64_t)c.heads * c.rows * G > INT32_MAX || (int64_t)c.batch * c.heads * ((c.cap + 127ll) / 128 * 128) > INT32_MAX)
+    return false;  // TMA coordinates
+  *bytes = kv4_tc_layout(c, G, t, nullptr);
+  return *bytes <= KV4_TC_BYTES;
+}
+
 // Query rows of a tile: 8 where every sequence's rows fit (one n8 tile of
 // the MMA), else 16, which unpacks a page once for twice the rows.
 static int ka_rows(int rows, int batch, int G) { return (int64_t)rows * G <= 8ll * batch ? 8 : 16; }
@@ -681,8 +722,13 @@ using namespace ltxb;
 extern "C" {
 
 uint64_t ltxb_attention_kv4_workspace_bytes(const ltxb_kv4_cache* cache, int rows, int H) {
-  if (!cache || rows <= 0 || H <= 0 || cache->kv_heads <= 0 || H % cache->kv_heads || cache->batch <= 0) return 0;
-  return ka_workspace(ka_rows(rows, cache->batch, H / cache->kv_heads));
+  Kv4View c;
+  Kv4Tc t;
+  if (rows <= 0 || H <= 0 || kv4_check(cache, nullptr, 0, "kv4 attention", &c) || H % c.heads || c.batch == 0) return 0;
+  c.rows = rows;
+  uint64_t bytes;
+  if (kv4_use_tc(c, H / c.heads, &bytes, &t)) return bytes;
+  return ka_workspace(ka_rows(rows, c.batch, H / c.heads));
 }
 
 int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, const void* q, int64_t ldq, void* out,
@@ -700,7 +746,10 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
   if (!(scale == scale) || scale - scale != 0.f) return set_error(LTXB_EINVAL, "kv4 attention: scale must be finite");
   a.G = H / cache->kv_heads;
   const int R = ka_rows(rows, cache->batch, a.G);
-  const uint64_t need = ka_workspace(R);
+  uint64_t need = 0;
+  Kv4Tc t{};
+  const bool tc = kv4_use_tc(a.c, a.G, &need, &t);
+  if (!tc) need = ka_workspace(R);
   if (!workspace || workspace_bytes < need)
     return set_error(LTXB_EINVAL, "kv4 attention: workspace of %llu bytes is smaller than the %llu required",
                      (unsigned long long)workspace_bytes, (unsigned long long)need);
@@ -711,9 +760,15 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
   a.out = static_cast<__nv_bfloat16*>(out);
   a.cs = scale * 1.4426950408889634f;
   a.causal = causal != 0;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (tc) {
+    kv4_tc_layout(a.c, a.G, &t, workspace);
+    t.cs = a.cs;
+    if (int rc = kv4_prepare(a.c, t, q, (size_t)ldq, cache->group, st)) return rc;
+    return kv4_attention_tc(a.c, t, gate, out, a.causal, st);
+  }
   a.cut = static_cast<int4*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)ka_ctas(R) * 16);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int ng = KV4_D / cache->group;
   if (R == 8) {
     if (ng == 1) return ka_launch<1, 8>(a, st);

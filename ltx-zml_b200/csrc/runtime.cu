@@ -247,6 +247,9 @@ int ltxb_device_status(int clear, uint32_t* site) {
   e = ltxb::attn_status(&va, clear != 0);
   if (e != cudaSuccess) return set_cuda_error(e, "read attention status");
   if (!v) v = va;
+  e = ltxb::kv4_attn_status(&va, clear != 0);
+  if (e != cudaSuccess) return set_cuda_error(e, "read attention status");
+  if (!v) v = va;
   uint32_t vi = 0;
   e = ltxb::index_status(&vi, clear != 0);
   if (e != cudaSuccess) return set_cuda_error(e, "read index status");

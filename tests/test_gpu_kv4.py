@@ -360,8 +360,7 @@ def test_bad_indexes_are_reported_and_not_followed(cuda):
         out = ltxb.attention_kv4(q.to(cuda), cache)
         rc, site = ltxb.device_status_site()
         assert rc == ltxb.EINVAL and site == ltxb.SITE_KV4_PAGE and "page" in ltxb.last_error()
-        keep = list(range(64)) + list(range(128, 130))
-        check(out[:1], kr.attention(q[:1], k[0][keep], v[0][keep], True), float(v[0].abs().max()))
+        assert bool(out[0].isnan().all())
         check(out[1:], kr.attention(q[1:], k[1], v[1], True), float(v[1].abs().max()))
         kk = rows_like((200, 2, 128), 1, cuda)
         before = cache.pages.clone()
@@ -457,3 +456,173 @@ def test_graph_replays_with_other_lengths_and_pages(cuda):
             kk, vv = (kr.held(torch.cat(t[b]).cpu(), group) for t in hist)
             check(out[b:b + 1], kr.attention(q[b:b + 1], kk, vv, True), float(vv.abs().max()), f"step {i}, {b}")
     assert ltxb.device_status() == ltxb.OK
+
+
+# ---------------------------------------------------------------------------
+# many rows: the tcgen05 kernel over f16 operands
+# ---------------------------------------------------------------------------
+
+def check_many(got, want, q, k, v, scale=None):
+    """K and V are rounded to f16 (2^-11 each), P too, exp2 is off by at most
+    2^-13: a score moves by at most 2^-11 scale sum |q_d k_d| =: 2^-11 A, so an
+    output by 2^-10 A max|v| from the scores (numerator and denominator) and
+    2^-9 max|v| from P, V and exp2, besides its own rounding. The roundings
+    being independent, the 2-norm of the error stays near that of the output's
+    rounding: bf16's root mean square error is at most 2^-8 / sqrt(3) = 2.3e-3
+    of a value; 3e-3 leaves room for the others (2^-11 / sqrt(3) each)."""
+    got = got.double().cpu()
+    if got.numel() == 0:
+        return
+    scale = 1 / math.sqrt(128) if scale is None else scale
+    a = scale * float((q.double().cpu().abs().amax((0, 1)) * k.abs().amax((0, 1))).sum())
+    vmax = float(v.abs().max())
+    err = (got - want).abs()
+    assert bool((err <= 2.0 ** -8 * want.abs() + vmax * (2.0 ** -9 + 2.0 ** -10 * a)).all())
+    n = float(want.norm())
+    assert float((got - want).norm()) <= 3e-3 * n, float((got - want).norm()) / n
+
+
+MANY = [
+    # lens, rows a sequence, H, Hkv, group, causal
+    ([64], 64, 1, 1, 128, True),
+    ([300], 300, 2, 1, 32, True),
+    ([257, 129], 128, 3, 3, 64, True),
+    ([500, 100, 130], 100, 4, 2, 128, False),
+    ([1000], 70, 7, 1, 32, True),          # 490 rows of one K/V head: a tile crosses tokens
+    ([1500], 256, 1, 1, 64, False),        # one tile: the keys are split
+    ([2000, 65], 65, 2, 2, 32, True),
+]
+
+
+@pytest.mark.parametrize("lens,new,H,Hkv,group,causal", MANY)
+def test_many_rows(cuda, lens, new, H, Hkv, group, causal):
+    import ltxb
+    cache, k, v = filled(lens, Hkv, group, cuda, seed=len(lens) + H)
+    q = torch.randn(len(lens) * new, H, 128, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16)
+    out = ltxb.attention_kv4(q.to(cuda), cache, causal=causal)
+    torch.cuda.synchronize()
+    assert ltxb.device_status() == ltxb.OK
+    for b in range(len(lens)):
+        qb = q[b * new:(b + 1) * new]
+        check_many(out[b * new:(b + 1) * new], kr.attention(qb, k[b], v[b], causal), qb, k[b], v[b])
+
+
+@pytest.mark.parametrize("scale", [0.2, -0.1, 0.0])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_ragged_rows(cuda, causal, scale):
+    """No rows, no tokens, fewer tokens than rows, one token; strided q, a gate, padding rows."""
+    import ltxb
+    lens, new, H, Hkv, group = [100, 0, 7, 300, 64, 3, 1, 513], [90, 20, 0, 300, 64, 50, 1, 200], 6, 2, 64
+    cache, k, v = filled(lens, Hkv, group, cuda, seed=4)
+    rs, n = starts(new, cuda), sum(new)
+    g = torch.Generator().manual_seed(10)
+    fused = torch.randn(n + 5, 2 * H, 128, generator=g).to(torch.bfloat16).to(cuda)
+    q = fused[:, H:]
+    gate = torch.rand(n + 5, H, generator=g).to(cuda)
+    out = torch.full((n + 5, H, 128), 5.0, dtype=torch.bfloat16, device=cuda)
+    ltxb.attention_kv4(q, cache, row_start=rs, causal=causal, gate=gate, scale=scale, out=out)
+    torch.cuda.synchronize()
+    assert ltxb.device_status() == ltxb.OK
+    at = 0
+    for b, c in enumerate(new):
+        if c:
+            qb = q[at:at + c].cpu()
+            want = kr.attention(qb, k[b], v[b], causal, scale=scale, gate=gate[at:at + c])
+            if lens[b]:
+                check_many(out[at:at + c], want, qb, k[b], v[b], scale=abs(scale))
+            # rows that see nothing are zeros, whole (a single value of another row may come to 0 as well)
+            assert torch.equal((out[at:at + c].cpu() == 0).all(-1), (want == 0).all(-1))
+        at += c
+    assert bool((out[n:] == 5).all())
+
+
+def test_many_rows_over_long_keys_in_splits(cuda):
+    import ltxb
+    lens, new, H, Hkv, group = [9000, 3001], [200, 90], 4, 2, 128
+    cache, k, v = filled(lens, Hkv, group, cuda, seed=1)
+    q = torch.randn(sum(new), H, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    for causal in (True, False):
+        out = ltxb.attention_kv4(q.to(cuda), cache, row_start=starts(new, cuda), causal=causal)
+        again = ltxb.attention_kv4(q.to(cuda), cache, row_start=starts(new, cuda), causal=causal)
+        assert torch.equal(out, again)
+        at = 0
+        for b, c in enumerate(new):
+            pick = list(range(0, c, 17)) + [c - 1]
+            for i in pick:
+                seen = lens[b] - c + i + 1 if causal else lens[b]
+                qi = q[at + i:at + i + 1]
+                want = kr.attention(qi, k[b][:seen], v[b][:seen], False)
+                check_many(out[at + i:at + i + 1], want, qi, k[b], v[b])
+            at += c
+    assert ltxb.device_status() == ltxb.OK
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_rows_nan_and_bad_pages(cuda, causal):
+    import ltxb
+    T, H = 300, 2
+    q = torch.randn(T, H, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    for which in ("k", "v", "page"):
+        k, v = rows_like((T, H, 128), 1, cuda), rows_like((T, H, 128), 2, cuda)
+        if which != "page":
+            (k if which == "k" else v)[130, 1, 17] = float("nan")
+        cache = make_cache([T], H, 32, cuda)
+        cache.append(k, v)
+        if which == "page":
+            cache.page_table[0, 2] = 1 << 20
+        out = ltxb.attention_kv4(q.to(cuda), cache, causal=causal).cpu()
+        assert ltxb.device_status() == (ltxb.EINVAL if which == "page" else ltxb.OK)
+        first = (128 if which == "page" else 130) if causal else 0
+        assert bool(out[first:, 1].isnan().all())
+        kh, vh = kr.held(k.cpu(), 32), kr.held(v.cpu(), 32)
+        heads = [0] if which != "page" else []
+        for h in heads:
+            check_many(out[:, h:h + 1], kr.attention(q[:, h:h + 1], kh[:, h:h + 1], vh[:, h:h + 1], causal),
+                       q[:, h:h + 1], kh[:, h:h + 1], vh[:, h:h + 1])
+        if causal:
+            check_many(out[:first, 1:], kr.attention(q[:first, 1:], kh[:first, 1:], vh[:first, 1:], True),
+                       q[:first, 1:], kh[:first, 1:], vh[:first, 1:])
+
+
+def test_many_rows_of_unequal_size(cuda):
+    """Rows, keys and values over many powers of two: the f16 operands' powers take them in."""
+    import ltxb
+    T, H = 200, 2
+    g = torch.Generator().manual_seed(3)
+    for qs, ks, vs in ((1e-30, 1e30, 1e-30), (1e25, 1e-25, 1e30), (1.0, 1.0, 1e-37), (1e-38, 1e-5, 1.0)):
+        q = (torch.randn(T, H, 128, generator=g) * qs * torch.exp2(torch.arange(T) % 5 - 2.0)[:, None, None]).to(torch.bfloat16)
+        k, v = (torch.randn(T, H, 128, generator=g) * s for s in (ks, vs))
+        k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+        cache = make_cache([T], H, 64, cuda)
+        cache.append(k.to(cuda), v.to(cuda))
+        out = ltxb.attention_kv4(q.to(cuda), cache)
+        kh, vh = kr.held(k, 64), kr.held(v, 64)
+        check_many(out, kr.attention(q, kh, vh, True), q, kh, vh)
+
+
+def test_capacity_far_above_the_lengths(cuda):
+    """A page table with room for 200 pages a sequence and a bound known on the host; lengths replayed in a graph."""
+    import ltxb
+    H, Hkv, group, new = 4, 2, 32, 48
+    cache = make_cache([100, 60], Hkv, group, cuda, max_pages=200)
+    bound = ltxb.KV4Cache.from_pages(cache.pages, cache.page_table, cache.seq_lens, group=group, max_len=700)
+    k, v = rows_like((1400, Hkv, 128), 1, cuda), rows_like((1400, Hkv, 128), 2, cuda)
+    cache.seq_lens.fill_(700)
+    cache.append(k, v)
+    kh, vh = kr.held(k.cpu(), group).view(2, 700, Hkv, 128), kr.held(v.cpu(), group).view(2, 700, Hkv, 128)
+    q = torch.randn(2 * new, H, 128, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).to(cuda)
+    out = torch.empty_like(q)
+    ltxb.attention_kv4(q, bound, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ltxb.attention_kv4(q, bound, out=out)
+    for lens in ([700, 699], [100, 48], [64, 640]):
+        cache.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        graph.replay()
+        for b, n in enumerate(lens):
+            qb = q[b * new:(b + 1) * new].cpu()
+            check_many(out[b * new:(b + 1) * new], kr.attention(qb, kh[b, :n], vh[b, :n], True), qb, kh[b, :n], vh[b, :n])
+    assert ltxb.device_status() == ltxb.OK
+    cache.seq_lens.fill_(701)
+    ltxb.attention_kv4(q, bound, out=out)
+    assert ltxb.device_status_site() == (ltxb.EINVAL, ltxb.SITE_KV4_LEN)
