@@ -1,35 +1,39 @@
 // Attention of a few query rows over the paged 4-bit K/V cache (decoding and
 // short runs of tokens): softmax(q k^T * scale) v with k, v = zero + scale_kv * code.
 //
-// The codes go to the tensor cores as they are. Put in the top mantissa bits
-// of a 16-bit float, a code c reads u = 1 + c / 16 exactly, and
-//   q . (z + s c)       = 16 s (q . u - 1.5 sum q) + (z + 8 s) sum q
-//   sum_t p_t (z + s c) = 16 (sum p s u - 1.5 sum p s) + sum p (z + 8 s)
-// (per group of 32 / 64 / 128 dims), so scale and zero touch only score-sized
-// data and unpacking costs one shift and one logic operation per two codes.
-// The offsets are subtracted where they were added: q's part as the initial
-// value of the accumulator, p's part by one more MMA with constant rows 1.5
-// over the same rounded p s.
+// The codes go to the tensor cores with almost no arithmetic. K: a code put
+// into the mantissa of an f16 reads u = 1 + c / 16 (mantissa bits 6-9) or
+// 1 + c / 256 (bits 2-5); q's values at the second kind of place are held 16
+// times larger, and the accumulator starts from -sum q (1 + 8 / 16 or
+// 1 + 8 / 256), so one shift and two logic operations unpack four codes and
+//   q . (z + s c) = 16 s acc + (z + 8 s) sum q,  acc = sum q (c - 8) / 16.
+// V: the sum over tokens is long, so its codes enter without an offset:
+// 1024 + c and 1024 + 16 c (mantissa bits 0-3 and 4-7) are taken to c - 8 by
+// one FMA each, exactly, and
+//   sum_t p_t (z + s c) = sum (p s) (c - 8) + sum p (z + 8 s).
+// Scale and zero thus touch only score-sized data (per group of 32 / 64 / 128).
 //
-// One warp takes 16 tokens of a page as the M side of mma.m16n8k16, so up to
-// 8 query rows (the query heads that share the K/V head, times the call's
+// A warp takes 16 tokens of a page as the M side of mma.m16n8k16, so up to 8
+// query rows (the query heads that share the K/V head, times the call's
 // tokens) cost the same as one: S^T = K Q^T, then O^T = V^T P^T with P^T
-// transposed in registers (movmatrix). K and q enter as bf16 (q is bf16, the
-// codes are exact). p s enters as f16 scaled by a power of two that follows
-// the largest V scale seen (between 2^3 and 2^7 times p): 11 significant bits
-// where bf16 would keep 8, so the result's own rounding dominates. Row maxima
-// move only when a score passes them by 2^8; sums and accumulators are f32.
+// transposed in registers (movmatrix). q enters as f16 after a power of two
+// per row (its 8 bits stay exact down to 2^-27 of the row's largest value).
+// p s enters as f16 scaled by a power of two that follows the largest V scale
+// seen (between 2^3 and 2^7 times p): 11 significant bits where bf16 would
+// keep 8, so the result's own rounding dominates. Row maxima move only when a
+// score passes them by 2^8; sums and accumulators are f32.
 //
 // Work is split by pages, not by sequence: all (sequence, head, row tile)
 // items laid end to end are one line of pages, each CTA takes an equal piece
-// of it, and a second kernel joins the items that were cut (in page order, so
-// results do not depend on timing). Lengths are read on the device only.
-// A page's block for one head (8.5 - 10 KB) arrives by one bulk copy into a
-// ring of KA_STAGES, so 4 CTAs keep about 100 KB per SM in flight.
+// of it, its warps take the pages of an item in turn, and a second kernel
+// joins the items that were cut (in page order, so results do not depend on
+// timing). Lengths are read on the device only. A warp has two slots of one
+// (page, head) block each, filled by one bulk copy (8.5 - 10 KB) while it
+// works on the other: no barrier between warps until an item ends.
 //
 // A token whose V group is stored as NaN, or whose page number is bad, makes
-// its score NaN (every row that attends to it becomes NaN) and is left out of
-// the product, so that rows which do not attend to it stay finite.
+// every row that attends to it NaN and no others: where a page holds tokens
+// that some row does not see, they are left out of the product.
 #include <float.h>
 
 #include <atomic>
@@ -38,8 +42,6 @@
 
 namespace ltxb {
 
-constexpr int KA_STAGES = 4;
-constexpr int KA_THREADS = 128;
 constexpr int KA_OLD = KV4_D + 4;  // floats per row of the warps' O tiles
 
 struct KaArgs {
@@ -61,13 +63,6 @@ __device__ __forceinline__ float ka_ex2(float x) {
   return y;
 }
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
   asm volatile(
@@ -86,17 +81,45 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// bf16 pair (1 + c / 16) of nibbles I and I + 4 of w
-template <int I>
-__device__ __forceinline__ uint32_t code_bf16(uint32_t w) {
-  const uint32_t s = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (s & 0x00780078u) | 0x3F803F80u;
+// K: from w << 2 (PART 0: nibbles 0, 4 and 1, 5) or w >> 6 (PART 1: nibbles 2,
+// 6 and 3, 7) the f16 pairs 1 + c / 256 (LO) or 1 + c / 16
+__device__ __forceinline__ uint32_t code_lo(uint32_t s) { return (s & 0x003C003Cu) | 0x3C003C00u; }
+__device__ __forceinline__ uint32_t code_hi(uint32_t s) { return (s & 0x03C003C0u) | 0x3C003C00u; }
+// V: the f16 pair c - 8 from bits 0-3 / 4-7 of both halves
+__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
 }
-// f16 pair (1 + c / 16) of nibble I of both halves of w
-template <int I>
-__device__ __forceinline__ uint32_t code_f16(uint32_t w) {
-  const uint32_t s = I < 2 ? w << (6 - 4 * I) : w >> (4 * I - 6);
-  return (s & 0x03C003C0u) | 0x3C003C00u;
+__device__ __forceinline__ uint32_t code_0(uint32_t w) {  // (1024 + c) - 1032
+  return h2_fma((w & 0x000F000Fu) | 0x64006400u, 0x3C003C00u, 0xE408E408u);
+}
+__device__ __forceinline__ uint32_t code_1(uint32_t w) {  // (1024 + 16 c) / 16 - 72
+  return h2_fma((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
+}
+// two-wide f32
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // One-dimensional bulk copy global -> shared; both ends 16-byte aligned, the
@@ -108,86 +131,104 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// A place on the line of pages: page `page` of (sequence b, row tile rt, head h).
-struct KaCursor {
-  int b, rt, h, page;
+// Pages [pa, pb) of (sequence b, row tile rt, head h): an item, or the part
+// of it that lies in a CTA's piece of the line of pages.
+struct KaSeg {
+  int b, rt, h, pa, pb;
   int pages, tiles, len, first, count;  // of sequence b
+  long long left;                       // pages of the CTA's piece from pa on
 };
 
 template <int R>
-__device__ __forceinline__ void ka_seq(const KaArgs& a, KaCursor& k) {
+__device__ __forceinline__ void ka_seq(const KaArgs& a, KaSeg& k) {
   k.len = kv4_len(a.c, k.b);
   kv4_rows(a.c, k.b, &k.first, &k.count);
   k.pages = (k.len + KV4_PAGE - 1) / KV4_PAGE;
   k.tiles = k.pages > 0 ? (k.count * a.G + R - 1) / R : 0;
 }
-
+__device__ __forceinline__ void ka_end(KaSeg& k) {
+  k.pb = k.pages - k.pa < k.left ? k.pages : k.pa + (int)k.left;
+}
+// The next item of the CTA's piece; false behind its last.
 template <int R>
-__device__ __forceinline__ void ka_next(const KaArgs& a, KaCursor& k) {
-  if (++k.page < k.pages) return;
-  k.page = 0;
-  if (++k.h < a.c.heads) return;
-  k.h = 0;
-  if (++k.rt < k.tiles) return;
-  k.rt = 0;
-  do {
-    if (++k.b >= a.c.batch) return;
-    ka_seq<R>(a, k);
-  } while (k.tiles == 0);
+__device__ __forceinline__ bool ka_next(const KaArgs& a, KaSeg& k) {
+  k.left -= k.pb - k.pa;
+  if (k.left <= 0) return false;
+  k.pa = 0;
+  if (++k.h >= a.c.heads) {
+    k.h = 0;
+    if (++k.rt >= k.tiles) {
+      k.rt = 0;
+      do {
+        if (++k.b >= a.c.batch) return false;
+        ka_seq<R>(a, k);
+      } while (k.tiles == 0);
+    }
+  }
+  ka_end(k);
+  return true;
 }
 
-template <int R>
+template <int NW, int R>
 struct KaSmem {
-  uint64_t full[KA_STAGES], empty[KA_STAGES];
-  int good[KA_STAGES];  // the stage's page number was valid
-  long long scan[4];
+  uint64_t full[NW][2];
+  int good[NW][2];  // the slot's page number was valid
+  long long scan[NW];
   int found[4];
-  float m[4][R], l[4][R];
-  float o[4][R][KA_OLD];
+  int busy[NW];     // the warp had pages of the item
+  float m[NW][R], l[NW][R];
 };
-template <int R>
+template <int NW, int R>
 constexpr int ka_smem_bytes(int ng) {
-  return KA_STAGES * kv4_block(ng) + (int)sizeof(KaSmem<R>) + 128;
+  return NW * 2 * kv4_block(ng) + (int)sizeof(KaSmem<NW, R>) + 128;
 }
+// Warps a CTA and CTAs an SM: as many warps as find two slots each in an
+// SM's 227 KB (12 of 8.5 or 9 KB, 10 of 10 KB).
+__host__ __device__ constexpr int ka_warps(int ng) { return ng == 4 ? 5 : 4; }
+__host__ __device__ constexpr int ka_per_sm(int ng) { return ng == 4 ? 2 : 3; }
 
 template <int NG, int R>
-__global__ void __launch_bounds__(KA_THREADS, R == 8 ? 4 : 3) kv4_attn_kernel(const KaArgs a) {
-  constexpr int NT = R / 8, BLK = kv4_block(NG);
+__global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_kernel(const KaArgs a) {
+  constexpr int NT = R / 8, BLK = kv4_block(NG), NW = ka_warps(NG), THREADS = NW * 32;
+  constexpr int MT = NG * NT <= 1 ? 4 : 2;  // tiles of 16 tokens whose scores are held at once
   extern __shared__ __align__(128) uint8_t ka_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ka_raw) + 127) & ~uintptr_t(127));
-  KaSmem<R>& sm = *reinterpret_cast<KaSmem<R>*>(ring + KA_STAGES * BLK);
+  KaSmem<NW, R>& sm = *reinterpret_cast<KaSmem<NW, R>*>(ring + NW * 2 * BLK);
+  static_assert(R * KA_OLD * 4 <= BLK, "a warp's O tile takes the place of a block");
   const int tid = threadIdx.x, warp = warp_id(), lane = lane_id(), g = lane >> 2, cq = lane & 3;
   const int Hq = a.c.heads * a.G;
 
   if (tid == 0) {
-    for (int i = 0; i < KA_STAGES; ++i) {
-      mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], 4);
+    for (int i = 0; i < NW; ++i) {
+      mbar_init(&sm.full[i][0], 1);
+      mbar_init(&sm.full[i][1], 1);
     }
     fence_mbar_init();
+    sm.found[0] = -1;
   }
-  // ---- this CTA's piece [u0, u1) of the line of pages ----
+  // ---- this CTA's piece of the line of pages ----
   auto units = [&](int b) -> long long {
-    KaCursor k;
+    KaSeg k;
     k.b = b;
     ka_seq<R>(a, k);
     return (long long)k.pages * k.tiles * a.c.heads;
   };
   long long mine = 0;
-  for (int b = tid; b < a.c.batch; b += KA_THREADS) mine += units(b);
+  for (int b = tid; b < a.c.batch; b += THREADS) mine += units(b);
 #pragma unroll
   for (int s = 16; s; s >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, s);
   if (lane == 0) sm.scan[warp] = mine;
-  if (tid == 0) sm.found[0] = -1;
   __syncthreads();
-  const long long total = sm.scan[0] + sm.scan[1] + sm.scan[2] + sm.scan[3];
+  long long total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) total += sm.scan[w];
   const int ctas = total < gridDim.x ? (int)total : (int)gridDim.x;
   // sequences without tokens: their rows attend to nothing and are zero
   for (int b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
     int first, count;
     kv4_rows(a.c, b, &first, &count);
     if (count > 0 && kv4_len(a.c, b) == 0)
-      for (long long i = tid; i < (long long)count * Hq * (KV4_D / 8); i += KA_THREADS)
+      for (long long i = tid; i < (long long)count * Hq * (KV4_D / 8); i += THREADS)
         reinterpret_cast<uint4*>(a.out + (size_t)first * Hq * KV4_D)[i] = make_uint4(0, 0, 0, 0);
   }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -196,11 +237,10 @@ __global__ void __launch_bounds__(KA_THREADS, R == 8 ? 4 : 3) kv4_attn_kernel(co
     return;
   }
   const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-  // the sequence that holds u0: prefix sums over 128 sequences at a time
-  KaCursor at;
-  {
+  KaSeg at;
+  {  // the sequence that holds u0: prefix sums over THREADS sequences at a time
     long long base = 0;
-    for (int b0 = 0;; b0 += KA_THREADS) {
+    for (int b0 = 0;; b0 += THREADS) {
       const long long n = b0 + tid < a.c.batch ? units(b0 + tid) : 0;
       long long x = n;
 #pragma unroll
@@ -215,7 +255,7 @@ __global__ void __launch_bounds__(KA_THREADS, R == 8 ? 4 : 3) kv4_attn_kernel(co
       x += base;
       if (n > 0 && u0 >= x - n && u0 < x) {
         const long long d = u0 - (x - n);
-        KaCursor k;
+        KaSeg k;
         k.b = b0 + tid;
         ka_seq<R>(a, k);
         sm.found[0] = k.b;
@@ -223,7 +263,8 @@ __global__ void __launch_bounds__(KA_THREADS, R == 8 ? 4 : 3) kv4_attn_kernel(co
         sm.found[2] = (int)(d / k.pages % a.c.heads);
         sm.found[3] = (int)(d % k.pages);
       }
-      base += sm.scan[0] + sm.scan[1] + sm.scan[2] + sm.scan[3];
+#pragma unroll
+      for (int w = 0; w < NW; ++w) base += sm.scan[w];
       if (base > u0 || b0 >= a.c.batch) break;
     }
     __syncthreads();
@@ -234,348 +275,411 @@ __global__ void __launch_bounds__(KA_THREADS, R == 8 ? 4 : 3) kv4_attn_kernel(co
     at.b = sm.found[0];
     at.rt = sm.found[1];
     at.h = sm.found[2];
-    at.page = sm.found[3];
+    at.pa = sm.found[3];
+    at.left = u1 - u0;
     ka_seq<R>(a, at);
+    ka_end(at);
   }
-  const int n = (int)(u1 - u0);
 
-  // ---- producer (lane 0 of warp 0): page i of this CTA into stage i % KA_STAGES ----
-  KaCursor pc = at;
-  int sent = 0;
+  // ---- loads: this warp's pages in order, alternately into its two slots (lane 0) ----
+  uint8_t* slots = ring + warp * 2 * BLK;
+  KaSeg ls = at;
+  int lp = at.pa + warp, sent = 0;
+  bool more = true;
   auto send = [&]() {
-    const int st = sent % KA_STAGES;
-    const int p = kv4_page(a.c, pc.b, pc.page);
-    sm.good[st] = p >= 0;
+    while (more && lp >= ls.pb) {
+      more = ka_next<R>(a, ls);
+      lp = ls.pa + warp;
+    }
+    if (!more) return;
+    const int p = kv4_page(a.c, ls.b, lp), st = sent & 1;
+    sm.good[warp][st] = p >= 0;
     if (p >= 0) {
-      mbar_arrive_expect_tx(&sm.full[st], BLK);
-      bulk_load(ring + st * BLK, kv4_block_at(a.c, p, pc.h, BLK), BLK, &sm.full[st]);
+      mbar_arrive_expect_tx(&sm.full[warp][st], BLK);
+      bulk_load(slots + st * BLK, kv4_block_at(a.c, p, ls.h, BLK), BLK, &sm.full[warp][st]);
     } else {
-      mbar_arrive(&sm.full[st]);
+      mbar_arrive(&sm.full[warp][st]);
     }
     ++sent;
-    if (sent < n) ka_next<R>(a, pc);
+    lp += NW;
   };
-  if (tid == 0)
-    while (sent < n && sent < KA_STAGES - 1) send();
+  if (lane == 0) {
+    send();
+    send();
+  }
+  __syncwarp();
 
-  bool ok = true, item = false, failed = false;
-  uint32_t qf[NT][16];
-  float qs[NT][NG][2], o[NT][8][4], o1[NT][NG][4], m[NT][2], l[NT][2], zs[NT][NG][2];
-  int lim[NT][2];
-  float sig = 1.f, sig_max = 0.f;  // p s is held as p * (s * sig); sig moves when s passes sig_max
-  int item_start = 0;              // page of the item this CTA began with
-  for (int i = 0; i < n; ++i) {
-    if (!item) {  // a new item: its query rows, and nothing accumulated
-      item = true;
-      item_start = at.page;
+  bool ok = true, failed = false, go = true;
+  int used = 0;  // pages this warp has taken from its slots
+  while (go) {
+    // ---- a new item: its query rows as f16, sums of q, nothing accumulated ----
+    uint32_t qf[NT][16];
+    uint64_t qs[NT][NG], rs[NT];      // rows 2 c, 2 c + 1: sum q per group; softmax scale * log2(e) / the row's power
+    float init[NT][NG][2];            // -sum q (1 + 8 / 16 or 1 + 8 / 256)
+    float o[NT][8][4], m[NT][2];
+    uint64_t l[NT], zs[NT][NG];
+    int lim[NT][2];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const int r = at.rt * R + t * 8 + g, tok = r / a.G;
-        const bool has = tok < at.count;
-        const __nv_bfloat16* src = a.q + (size_t)(at.first + tok) * a.ldq + (at.h * a.G + (r - tok * a.G)) * KV4_D + 8 * cq;
+    for (int t = 0; t < NT; ++t) {
+      const int r = at.rt * R + t * 8 + g, tok = r / a.G;
+      const bool has = tok < at.count;
+      const __nv_bfloat16* src =
+          a.q + (size_t)(at.first + (has ? tok : 0)) * a.ldq + (at.h * a.G + (has ? r - tok * a.G : 0)) * KV4_D + 8 * cq;
+      uint4 w[4];
+      float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint4 w = has ? __ldg(reinterpret_cast<const uint4*>(src + 32 * j)) : make_uint4(0, 0, 0, 0);
-          qf[t][4 * j + 0] = __byte_perm(w.x, w.z, 0x5410);  // dims 0, 4 of the eight
-          qf[t][4 * j + 1] = __byte_perm(w.x, w.z, 0x7632);  // 1, 5
-          qf[t][4 * j + 2] = __byte_perm(w.y, w.w, 0x5410);  // 2, 6
-          qf[t][4 * j + 3] = __byte_perm(w.y, w.w, 0x7632);  // 3, 7
-        }
+      for (int j = 0; j < 4; ++j) {
+        w[j] = has ? __ldg(reinterpret_cast<const uint4*>(src + 32 * j)) : make_uint4(0, 0, 0, 0);
+        const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int rc = at.rt * R + t * 8 + 2 * cq + e, tc = rc / a.G;
-          lim[t][e] = a.causal ? at.len - at.count + tc : at.len - 1;  // last key the row sees
-          m[t][e] = -FLT_MAX;
-          l[t][e] = 0.f;
-        }
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[t][x][e] = 0.f;
-#pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int y = 0; y < 8 / NG; ++y) {
-            const int k = x * (8 / NG) + y;
-            mma_bf16(s, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u, qf[t][2 * k], qf[t][2 * k + 1]);
-          }
-          qs[t][x][0] = s[0];
-          qs[t][x][1] = s[1];
-          zs[t][x][0] = zs[t][x][1] = 0.f;
-          o1[t][x][0] = o1[t][x][1] = o1[t][x][2] = o1[t][x][3] = 0.f;
-        }
+        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(ws[i])), fabsf(bf16_hi(ws[i]))));
       }
-      sig = 1.f;
-      sig_max = 0.f;
-    }
-    const int st = i % KA_STAGES;
-    if (ok) ok = warp_wait(&sm.full[st], (i / KA_STAGES) & 1, 0x301);
-    if (ok) {
-      const uint8_t* blk = ring + st * BLK;
-      const int t0 = warp * 16 + g;  // this lane's tokens t0 and t0 + 8 of the page
-      const int key0 = at.page * KV4_PAGE + t0, key1 = key0 + 8;
-      const int len = at.len;
-      const bool good = sm.good[st] != 0;
-      // ---- S^T: 16 tokens x R rows ----
-      float s[NT][4];
-      {
-        const uint4 k0 = *reinterpret_cast<const uint4*>(blk + t0 * 64 + cq * 16);
-        const uint4 k1 = *reinterpret_cast<const uint4*>(blk + (t0 + 8) * 64 + cq * 16);
-        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-        float acc[NT][NG][4];
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int field = 264 - (int)(__float_as_uint(top) >> 23);  // the largest value into [2^10, 2^11)
+      field = field < 1 ? 1 : field > 249 ? 249 : field;
+      const float f = __uint_as_float((uint32_t)field << 23), f16 = 16.f * f;
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int x = 0; x < NG; ++x) {
-            acc[t][x][0] = acc[t][x][2] = -1.5f * qs[t][x][0];
-            acc[t][x][1] = acc[t][x][3] = -1.5f * qs[t][x][1];
-          }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int x = j * NG / 4;
-          const uint32_t a00 = code_bf16<0>(w0[j]), a10 = code_bf16<0>(w1[j]), a01 = code_bf16<1>(w0[j]),
-                         a11 = code_bf16<1>(w1[j]), a02 = code_bf16<2>(w0[j]), a12 = code_bf16<2>(w1[j]),
-                         a03 = code_bf16<3>(w0[j]), a13 = code_bf16<3>(w1[j]);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            mma_bf16(acc[t][x], a00, a10, a01, a11, qf[t][4 * j], qf[t][4 * j + 1]);
-            mma_bf16(acc[t][x], a02, a12, a03, a13, qf[t][4 * j + 2], qf[t][4 * j + 3]);
-          }
-        }
-        const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + KV4_KPAIR);
-#pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
-#pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          const uint32_t p0 = kp[t0 * NG + x], p1 = kp[(t0 + 8) * NG + x];
-          const float s0 = bf16_lo(p0) * a.cs, s1 = bf16_lo(p1) * a.cs;
-          const float z0 = fmaf(8.f, s0, bf16_hi(p0) * a.cs), z1 = fmaf(8.f, s1, bf16_hi(p1) * a.cs);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            s[t][0] += fmaf(16.f * s0, acc[t][x][0], z0 * qs[t][x][0]);
-            s[t][1] += fmaf(16.f * s0, acc[t][x][1], z0 * qs[t][x][1]);
-            s[t][2] += fmaf(16.f * s1, acc[t][x][2], z1 * qs[t][x][0]);
-            s[t][3] += fmaf(16.f * s1, acc[t][x][3], z1 * qs[t][x][1]);
-          }
-        }
+      for (int j = 0; j < 4; ++j) {
+        qf[t][4 * j + 0] = pack_f16x2(bf16_lo(w[j].x) * f16, bf16_lo(w[j].z) * f16);  // dims 0, 4 of the eight
+        qf[t][4 * j + 1] = pack_f16x2(bf16_hi(w[j].x) * f, bf16_hi(w[j].z) * f);      // 1, 5
+        qf[t][4 * j + 2] = pack_f16x2(bf16_lo(w[j].y) * f16, bf16_lo(w[j].w) * f16);  // 2, 6
+        qf[t][4 * j + 3] = pack_f16x2(bf16_hi(w[j].y) * f, bf16_hi(w[j].w) * f);      // 3, 7
       }
-      // ---- V scales of the two tokens: sv = 16 s, zv = z + 8 s ----
-      float sv0[NG], sv1[NG], zv0[NG], zv1[NG], bad0 = 0.f, bad1 = 0.f, svm = 0.f;
-      {
-        const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + kv4_vpair(NG));
+      const float back = __uint_as_float((uint32_t)(254 - field) << 23) * a.cs;
+      rs[t] = f2(__shfl_sync(0xffffffffu, back, 8 * cq), __shfl_sync(0xffffffffu, back, 8 * cq + 4));
 #pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          const uint32_t p0 = vp[t0 * NG + x], p1 = vp[(t0 + 8) * NG + x];
-          sv0[x] = bf16_lo(p0);
-          sv1[x] = bf16_lo(p1);
-          zv0[x] = fmaf(8.f, sv0[x], bf16_hi(p0));
-          zv1[x] = fmaf(8.f, sv1[x], bf16_hi(p1));
-          // a group that is not finite, a page that was not read, a token behind
-          // the last one (which the mask takes out): not in the product
-          if (key0 >= len || !good || !(fabsf(zv0[x]) < INFINITY)) {
-            bad0 = NAN;
-            sv0[x] = zv0[x] = 0.f;
-          }
-          if (key1 >= len || !good || !(fabsf(zv1[x]) < INFINITY)) {
-            bad1 = NAN;
-            sv1[x] = zv1[x] = 0.f;
-          }
-          svm = fmaxf(svm, fmaxf(sv0[x], sv1[x]));
-        }
+      for (int e = 0; e < 2; ++e) {
+        const int rc = at.rt * R + t * 8 + 2 * cq + e;
+        lim[t][e] = a.causal ? at.len - at.count + rc / a.G : at.len - 1;  // last key the row sees
+        m[t][e] = -FLT_MAX;
       }
-      // ---- masks; reference maxima and the V power move only when they must ----
-      bool move = svm > sig_max;
+      l[t] = 0;
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int x = 0; x < 8; ++x)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int last = lim[t][e] < len - 1 ? lim[t][e] : len - 1;
-          s[t][e] = key0 <= last ? s[t][e] + bad0 : -INFINITY;
-          s[t][2 + e] = key1 <= last ? s[t][2 + e] + bad1 : -INFINITY;
-          move = move || fmaxf(s[t][e], s[t][2 + e]) > m[t][e] + 8.f;
+        for (int e = 0; e < 4; ++e) o[t][x][e] = 0.f;
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        float s[4] = {0.f, 0.f, 0.f, 0.f}, n[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int y = 0; y < 8 / NG; ++y) {
+          const int k = x * (8 / NG) + y;
+          mma_f16(s, 0x2C002C00u, 0x2C002C00u, 0x3C003C00u, 0x3C003C00u, qf[t][2 * k], qf[t][2 * k + 1]);
+          mma_f16(n, 0xBC20BC20u, 0xBC20BC20u, 0xBE00BE00u, 0xBE00BE00u, qf[t][2 * k], qf[t][2 * k + 1]);
         }
-      if (__any_sync(0xffffffffu, move)) {
-#pragma unroll
-        for (int k = 4; k < 32; k <<= 1) svm = fmaxf(svm, __shfl_xor_sync(0xffffffffu, svm, k));
-        float turn = 1.f;
-        if (svm > sig_max) {  // the same in every lane
-          // sig = 2^(3 - floor(log2 svm)): s * sig in [8, 16) now, at most 128 before it moves again
-          int ex = 257 - (int)(__float_as_uint(svm) >> 23);
-          ex = ex > 253 ? 253 : ex < 1 ? 1 : ex;
-          const float ns = __uint_as_float((uint32_t)ex << 23);
-          turn = ns / sig;
-          sig = ns;
-          sig_max = 128.f / ns;
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float f[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float top = fmaxf(m[t][e], fmaxf(s[t][e], s[t][2 + e]));
-#pragma unroll
-            for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-            const float c = ka_ex2(m[t][e] - top);
-            m[t][e] = top;
-            l[t][e] *= c;
-#pragma unroll
-            for (int x = 0; x < NG; ++x) zs[t][x][e] *= c;
-            f[e] = c * turn;
-          }
-#pragma unroll
-          for (int x = 0; x < 8; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[t][x][e] *= f[e & 1];
-#pragma unroll
-          for (int x = 0; x < NG; ++x)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o1[t][x][e] *= f[e & 1];
-        }
-      }
-      // ---- p, its sums, and P^T fragments ----
-      uint32_t pb[NT][NG][2];
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        float p[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) p[e] = ka_ex2(s[t][e] - m[t][e & 1]);
-        l[t][0] += p[0] + p[2];
-        l[t][1] += p[1] + p[3];
-#pragma unroll
-        for (int x = 0; x < NG; ++x) {
-          zs[t][x][0] += fmaf(p[0], zv0[x], p[2] * zv1[x]);
-          zs[t][x][1] += fmaf(p[1], zv0[x], p[3] * zv1[x]);
-          const float f0 = sv0[x] * sig, f1 = sv1[x] * sig;
-          pb[t][x][0] = transpose8x8(pack_f16x2(p[0] * f0, p[1] * f0));
-          pb[t][x][1] = transpose8x8(pack_f16x2(p[2] * f1, p[3] * f1));
-        }
-      }
-      // ---- O^T += V^T P^T ----
-      {
-        const uint8_t* vb = blk + KV4_VOFF + warp * 1024 + lane * 16;
-        const uint4 v0 = *reinterpret_cast<const uint4*>(vb), v1 = *reinterpret_cast<const uint4*>(vb + 512);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int x = j * NG / 4;
-          const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
-          const uint32_t w0 = __byte_perm(j < 2 ? v0.x : v0.y, j < 2 ? v0.z : v0.w, sel);
-          const uint32_t w1 = __byte_perm(j < 2 ? v1.x : v1.y, j < 2 ? v1.z : v1.w, sel);
-          const uint32_t a00 = code_f16<0>(w0), a01 = code_f16<1>(w0), a02 = code_f16<2>(w0), a03 = code_f16<3>(w0);
-          const uint32_t a10 = code_f16<0>(w1), a11 = code_f16<1>(w1), a12 = code_f16<2>(w1), a13 = code_f16<3>(w1);
-#pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            mma_f16(o[t][2 * j], a00, a01, a10, a11, pb[t][x][0], pb[t][x][1]);
-            mma_f16(o[t][2 * j + 1], a02, a03, a12, a13, pb[t][x][0], pb[t][x][1]);
-          }
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int x = 0; x < NG; ++x)
-            mma_f16(o1[t][x], 0x3E003E00u, 0x3E003E00u, 0x3E003E00u, 0x3E003E00u, pb[t][x][0], pb[t][x][1]);
+        qs[t][x] = f2(s[0], s[1]);
+        init[t][x][0] = n[0];
+        init[t][x][1] = n[1];
+        zs[t][x] = 0;
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&sm.empty[st]);
-    if (tid == 0 && sent < n) {  // the stage that page i - 1 has left
-      bool fre = true;
-      if (i > 0) fre = mbar_wait(&sm.empty[(i - 1) % KA_STAGES], ((i - 1) / KA_STAGES) & 1, 0x302);
-      if (fre)
-        send();
-      else
-        ok = false;
-    }
-    __syncwarp();
-    const bool last_page = at.page + 1 == at.pages;
-    if (last_page || i + 1 == n) {
-      // ---- the item ends here, or this CTA's piece of it: join the warps ----
-      failed = __syncthreads_or(!ok);  // also: the last item's tiles have been read
-      if (failed) break;
+    // keys that every row of the tile sees: up to the first row's
+    const int all = a.causal ? at.len - at.count + (at.rt * R) / a.G : at.len - 1;
+    float sig = 1.f, sig_max = 0.f;  // p s is held as p * (s * sig); sig moves when s passes sig_max
+    const int npg = at.pb - at.pa > warp ? (at.pb - at.pa - warp + NW - 1) / NW : 0;
+    for (int k = 0; k < npg; ++k, ++used) {
+      const int st = used & 1;
+      if (ok) ok = warp_wait(&sm.full[warp][st], (used >> 1) & 1, 0x301);
+      if (!ok) break;
+      const uint8_t* blk = slots + st * BLK;
+      const int page = at.pa + warp + k * NW;
+      const bool good = sm.good[warp][st] != 0;
+      const bool whole = good && page * KV4_PAGE + KV4_PAGE - 1 <= all;
+#pragma unroll 1
+      for (int h = 0; h < 4 / MT; ++h) {
+        uint64_t s[MT][NT][2];
+        float svm = 0.f;
+        const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + kv4_vpair(NG)) + (h * MT * 16 + g) * NG;
+        // ---- S^T of MT tiles: 16 tokens x R rows each, lane: tokens g, g + 8, rows 2 c, 2 c + 1 ----
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const float back = 16.f / sig;
+        for (int mt = 0; mt < MT; ++mt) {
+          const int t0 = (h * MT + mt) * 16 + g;
+          const uint4 k0 = *reinterpret_cast<const uint4*>(blk + t0 * 64 + cq * 16);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(blk + (t0 + 8) * 64 + cq * 16);
+          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          float acc[NT][NG][4];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int k = 4; k < 32; k <<= 1) {
-            l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], k);
-#pragma unroll
-            for (int x = 0; x < NG; ++x) zs[t][x][e] += __shfl_xor_sync(0xffffffffu, zs[t][x][e], k);
-          }
-          const int r = t * 8 + 2 * cq + e;
-          if (g == 0) {
-            sm.m[warp][r] = m[t][e];
-            sm.l[warp][r] = l[t][e];
-          }
+            for (int x = 0; x < NG; ++x) {
+              acc[t][x][0] = acc[t][x][2] = init[t][x][0];
+              acc[t][x][1] = acc[t][x][3] = init[t][x][1];
+            }
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const int x = j * NG / 4;
-            const float c1 = o1[t][x][e], z = zs[t][x][e];
-            *reinterpret_cast<float4*>(&sm.o[warp][r][32 * j + 4 * g]) =
-                make_float4(fmaf(o[t][2 * j][e] - c1, back, z), fmaf(o[t][2 * j][2 + e] - c1, back, z),
-                            fmaf(o[t][2 * j + 1][e] - c1, back, z), fmaf(o[t][2 * j + 1][2 + e] - c1, back, z));
+            const uint32_t a0 = w0[j] << 2, a1 = w1[j] << 2, b0 = w0[j] >> 6, b1 = w1[j] >> 6;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              mma_f16(acc[t][x], code_lo(a0), code_lo(a1), code_hi(a0), code_hi(a1), qf[t][4 * j], qf[t][4 * j + 1]);
+              mma_f16(acc[t][x], code_lo(b0), code_lo(b1), code_hi(b0), code_hi(b1), qf[t][4 * j + 2], qf[t][4 * j + 3]);
+            }
+          }
+          const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + KV4_KPAIR) + t0 * NG;
+#pragma unroll
+          for (int x = 0; x < NG; ++x) {
+            const uint32_t p0 = kp[x], p1 = kp[8 * NG + x];
+            const float s0 = bf16_lo(p0), s1 = bf16_lo(p1);
+            const float z0 = fmaf(8.f, s0, bf16_hi(p0)), z1 = fmaf(8.f, s1, bf16_hi(p1));
+            const float a0 = 16.f * s0, a1 = 16.f * s1;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              uint64_t y0 = f2mul(f2(z0, z0), qs[t][x]), y1 = f2mul(f2(z1, z1), qs[t][x]);
+              if (x > 0) {
+                y0 = f2add(y0, s[mt][t][0]);
+                y1 = f2add(y1, s[mt][t][1]);
+              }
+              s[mt][t][0] = f2fma(f2(a0, a0), f2(acc[t][x][0], acc[t][x][1]), y0);
+              s[mt][t][1] = f2fma(f2(a1, a1), f2(acc[t][x][2], acc[t][x][3]), y1);
+            }
+            svm = fmaxf(svm, fmaxf(bf16_lo(vp[mt * 16 * NG + x]), bf16_lo(vp[(mt * 16 + 8) * NG + x])));
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            s[mt][t][0] = f2mul(s[mt][t][0], rs[t]);
+            s[mt][t][1] = f2mul(s[mt][t][1], rs[t]);
+          }
+        }
+        // ---- a page that holds tokens some row does not see ----
+        if (!whole) {
+          svm = 0.f;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const int key = page * KV4_PAGE + (h * MT + mt) * 16 + y * 8 + g;
+              float bad = good ? 0.f : NAN;  // NaN for a row that sees a token which is not finite
+              const bool in = key < at.len && good;
+#pragma unroll
+              for (int x = 0; x < NG; ++x) {
+                const uint32_t p = vp[(mt * 16 + y * 8) * NG + x];
+                const float z = fmaf(8.f, bf16_lo(p), bf16_hi(p));
+                if (!(fabsf(z) < INFINITY))
+                  bad = NAN;
+                else if (in)
+                  svm = fmaxf(svm, bf16_lo(p));
+              }
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                float x0, x1;
+                un2(s[mt][t][y], x0, x1);
+                x0 = key <= lim[t][0] && key < at.len ? x0 + bad : -INFINITY;
+                x1 = key <= lim[t][1] && key < at.len ? x1 + bad : -INFINITY;
+                s[mt][t][y] = f2(x0, x1);
+              }
+            }
+        }
+        // ---- reference maxima and the V power move only when they must ----
+        bool move = svm > sig_max;
+        float top[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            float x0, x1, x2, x3;
+            un2(s[mt][t][0], x0, x1);
+            un2(s[mt][t][1], x2, x3);
+            top[t][0] = mt ? fmaxf(top[t][0], fmaxf(x0, x2)) : fmaxf(x0, x2);
+            top[t][1] = mt ? fmaxf(top[t][1], fmaxf(x1, x3)) : fmaxf(x1, x3);
+          }
+          move = move || top[t][0] > m[t][0] + 8.f || top[t][1] > m[t][1] + 8.f;
+        }
+        if (__any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) svm = fmaxf(svm, __shfl_xor_sync(0xffffffffu, svm, i));
+          float turn = 1.f;
+          if (svm > sig_max) {  // the same in every lane
+            // sig = 2^(3 - floor(log2 svm)): s * sig in [8, 16) now, at most 128 before it moves again
+            int ex = 257 - (int)(__float_as_uint(svm) >> 23);
+            ex = ex > 253 ? 253 : ex < 1 ? 1 : ex;
+            const float ns = __uint_as_float((uint32_t)ex << 23);
+            turn = ns / sig;
+            sig = ns;
+            sig_max = 128.f / ns;
+          }
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            float c[2], f[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(m[t][e], top[t][e]);
+#pragma unroll
+              for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
+              c[e] = ka_ex2(m[t][e] - x);
+              m[t][e] = x;
+              f[e] = c[e] * turn;
+            }
+            l[t] = f2mul(l[t], f2(c[0], c[1]));
+#pragma unroll
+            for (int x = 0; x < NG; ++x) zs[t][x] = f2mul(zs[t][x], f2(c[0], c[1]));
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[t][x][e] *= f[e & 1];
+          }
+        }
+        // ---- p, its sums, P^T fragments, O^T += V^T P^T ----
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t pb[NT][NG][2];
+          uint64_t p2[NT][2];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const uint64_t nm = f2(-m[t][0], -m[t][1]);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float x0, x1;
+              un2(f2add(s[mt][t][y], nm), x0, x1);
+              p2[t][y] = f2(ka_ex2(x0), ka_ex2(x1));
+              l[t] = f2add(l[t], p2[t][y]);
+            }
+          }
+#pragma unroll
+          for (int x = 0; x < NG; ++x)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t p = vp[(mt * 16 + y * 8) * NG + x];
+              float sv = bf16_lo(p), zv = fmaf(8.f, sv, bf16_hi(p));
+              if (!whole) {
+                const int key = page * KV4_PAGE + (h * MT + mt) * 16 + y * 8 + g;
+                if (key >= at.len || !good || !(fabsf(zv) < INFINITY)) sv = zv = 0.f;
+              }
+              const float f = sv * sig;
+#pragma unroll
+              for (int t = 0; t < NT; ++t) {
+                zs[t][x] = f2fma(p2[t][y], f2(zv, zv), zs[t][x]);
+                float x0, x1;
+                un2(f2mul(p2[t][y], f2(f, f)), x0, x1);
+                pb[t][x][y] = transpose8x8(pack_f16x2(x0, x1));
+              }
+            }
+          const uint8_t* vb = blk + KV4_VOFF + (h * MT + mt) * 1024 + lane * 16;
+          const uint4 v0 = *reinterpret_cast<const uint4*>(vb), v1 = *reinterpret_cast<const uint4*>(vb + 512);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int x = j * NG / 4;
+            const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
+            const uint32_t w0 = __byte_perm(j < 2 ? v0.x : v0.y, j < 2 ? v0.z : v0.w, sel);
+            const uint32_t w1 = __byte_perm(j < 2 ? v1.x : v1.y, j < 2 ? v1.z : v1.w, sel);
+            const uint32_t a0 = code_0(w0), a1 = code_1(w0), a2 = code_0(w1), a3 = code_1(w1);
+            const uint32_t b0 = code_0(w0 >> 8), b1 = code_1(w0 >> 8), b2 = code_0(w1 >> 8), b3 = code_1(w1 >> 8);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              mma_f16(o[t][2 * j], a0, a1, a2, a3, pb[t][x][0], pb[t][x][1]);
+              mma_f16(o[t][2 * j + 1], b0, b1, b2, b3, pb[t][x][0], pb[t][x][1]);
+            }
           }
         }
       }
-      __syncthreads();
-      const bool whole = item_start == 0 && last_page;
-      float* slot = a.part + (size_t)(2 * blockIdx.x + (item_start == 0 ? 1 : 0)) * (R * (KV4_D + 2));
-#pragma unroll 1
-      for (int r = warp; r < R; r += 4) {
-        const int rr = at.rt * R + r, tok = rr / a.G, head = at.h * a.G + (rr - tok * a.G);
-        if (tok >= at.count) break;
-        const float top = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
-        float sum = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      __syncwarp();
+      if (lane == 0 && k + 1 < npg) send();  // the last page's slot serves as this warp's O tile first
+      __syncwarp();
+    }
+    // ---- the item, or this CTA's piece of it, is done: join the warps ----
+    float* ot = reinterpret_cast<float*>(slots + ((used - 1) & 1) * BLK);  // with pages only: the slot just read
+    if (ok && npg > 0) {
+      const float back = 1.f / sig;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+      for (int t = 0; t < NT; ++t) {
+        float lt[2], z[NG][2];
+        un2(l[t], lt[0], lt[1]);
+#pragma unroll
+        for (int x = 0; x < NG; ++x) un2(zs[t][x], z[x][0], z[x][1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int i = 4; i < 32; i <<= 1) {
+            lt[e] += __shfl_xor_sync(0xffffffffu, lt[e], i);
+#pragma unroll
+            for (int x = 0; x < NG; ++x) z[x][e] += __shfl_xor_sync(0xffffffffu, z[x][e], i);
+          }
+          // a NaN group of any V makes the whole row NaN, not its own dims alone
+#pragma unroll
+          for (int x = 0; x < NG; ++x) lt[e] += z[x][e] - z[x][e];
+          const int r = t * 8 + 2 * cq + e;
+          if (g == 0) {
+            sm.m[warp][r] = m[t][e];
+            sm.l[warp][r] = lt[e];
+          }
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float zz = z[j * NG / 4][e];
+            *reinterpret_cast<float4*>(ot + r * KA_OLD + 32 * j + 4 * g) =
+                make_float4(fmaf(o[t][2 * j][e], back, zz), fmaf(o[t][2 * j][2 + e], back, zz),
+                            fmaf(o[t][2 * j + 1][e], back, zz), fmaf(o[t][2 * j + 1][2 + e], back, zz));
+          }
+        }
+      }
+    }
+    if (lane == 0) sm.busy[warp] = npg > 0 ? 1 + ((used - 1) & 1) : 0;  // 1 + the slot that holds the O tile
+    failed = __syncthreads_or(!ok);
+    if (failed) break;
+    const bool ends = at.pb == at.pages, whole_item = ends && at.pa == 0;
+    float* slot = a.part + (size_t)(2 * blockIdx.x + (at.pa == 0 ? 1 : 0)) * (R * (KV4_D + 2));
+#pragma unroll 1
+    for (int r = warp; r < R; r += NW) {
+      const int rr = at.rt * R + r, tok = rr / a.G, head = at.h * a.G + (rr - tok * a.G);
+      if (tok >= at.count) break;
+      float top = -FLT_MAX;
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+        if (sm.busy[w]) top = fmaxf(top, sm.m[w][r]);
+      float sum = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < NW; ++w)
+        if (sm.busy[w]) {
           const float f = ka_ex2(sm.m[w][r] - top);
-          const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][r][4 * lane]);
+          const float4 x = *reinterpret_cast<const float4*>(ring + (w * 2 + sm.busy[w] - 1) * BLK + (r * KA_OLD + 4 * lane) * 4);
           sum = fmaf(sm.l[w][r], f, sum);
           v.x = fmaf(x.x, f, v.x);
           v.y = fmaf(x.y, f, v.y);
           v.z = fmaf(x.z, f, v.z);
           v.w = fmaf(x.w, f, v.w);
         }
-        if (whole) {
-          const size_t orow = (size_t)(at.first + tok) * Hq + head;
-          const float f = (sum == 0.f ? 0.f : 1.f / sum) * (a.gate ? __ldg(a.gate + orow) : 1.f);
-          *reinterpret_cast<uint2*>(a.out + orow * KV4_D + 4 * lane) =
-              make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
-        } else {
-          *reinterpret_cast<float4*>(slot + r * KV4_D + 4 * lane) = v;
-          if (lane == 0) {
-            slot[R * KV4_D + r] = top;
-            slot[R * KV4_D + R + r] = sum;
-          }
+      if (whole_item) {
+        const size_t orow = (size_t)(at.first + tok) * Hq + head;
+        const float f = (sum == 0.f ? 0.f : 1.f / sum) * (a.gate ? __ldg(a.gate + orow) : 1.f);
+        *reinterpret_cast<uint2*>(a.out + orow * KV4_D + 4 * lane) =
+            make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+      } else {
+        *reinterpret_cast<float4*>(slot + r * KV4_D + 4 * lane) = v;
+        if (lane == 0) {
+          slot[R * KV4_D + r] = top;
+          slot[R * KV4_D + R + r] = sum;
         }
       }
-      if (i + 1 == n && tid == 0) {
-        int4 cut = make_int4(-1, 0, 0, 0);
-        if (item_start == 0 && !last_page) {
-          // its last page is page u1 - 1 + (pages - 1 - at.page) of the line
-          const long long end = u1 - 1 + (at.pages - 1 - at.page);
-          long long z = (end * ctas) / total;
-          while (total * (z + 1) / ctas <= end) ++z;
-          while (total * z / ctas > end) --z;
-          cut = make_int4(at.b, at.rt, at.h, (int)z);
-        }
-        a.cut[blockIdx.x] = cut;
-      }
-      item = false;
     }
-    if (i + 1 < n) ka_next<R>(a, at);
+    const KaSeg was = at;
+    go = ka_next<R>(a, at);
+    if (!go && tid == 0) {
+      int4 cut = make_int4(-1, 0, 0, 0);
+      if (was.pa == 0 && !ends) {
+        // the item's last page on the line of pages, and the CTA that has it
+        const long long end = u1 - 1 + (was.pages - was.pb);
+        long long z = (end * ctas) / total;
+        while (total * (z + 1) / ctas <= end) ++z;
+        while (total * z / ctas > end) --z;
+        cut = make_int4(was.b, was.rt, was.h, (int)z);
+      }
+      a.cut[blockIdx.x] = cut;
+    }
+    fence_proxy_async_smem();  // the O tiles were written and read as ordinary memory; copies follow
+    __syncthreads();
+    if (lane == 0 && npg > 0) send();
+    __syncwarp();
   }
   // a failed wait (reported in the status word) leaves copies under way: let
   // them land before this CTA's shared memory is given up
-  if (tid == 0) {
-    const uint64_t t0 = globaltimer_ns();
-    for (int i = sent > KA_STAGES ? sent - KA_STAGES : 0; i < sent; ++i)
-      while (!mbar_try_wait(smem_u32(&sm.full[i % KA_STAGES]), (i / KA_STAGES) & 1) &&
-             globaltimer_ns() - t0 < kWaitLimitNs) {
-      }
-    if (failed) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+  if (failed) {
+    if (lane == 0) {
+      const uint64_t t0 = globaltimer_ns();
+      for (int i = used; i < sent; ++i)
+        while (!mbar_try_wait(smem_u32(&sm.full[warp][i & 1]), (i >> 1) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
+        }
+    }
+    if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
 }
 
@@ -678,15 +782,15 @@ static bool kv4_use_tc(const Kv4View& c, int G, uint64_t* bytes, Kv4Tc* t) {
 // Query rows of a tile: 8 where every sequence's rows fit (one n8 tile of
 // the MMA), else 16, which unpacks a page once for twice the rows.
 static int ka_rows(int rows, int batch, int G) { return (int64_t)rows * G <= 8ll * batch ? 8 : 16; }
-static int ka_ctas(int R) { return sm_count() * (R == 8 ? 4 : 3); }
-static uint64_t ka_workspace(int R) {
-  const uint64_t n = ka_ctas(R);
+static int ka_ctas(int group) { return sm_count() * ka_per_sm(KV4_D / group); }
+static uint64_t ka_workspace(int R, int group) {
+  const uint64_t n = ka_ctas(group);
   return n * 16 + n * 2 * R * (KV4_D + 2) * 4;
 }
 
 template <int NG, int R>
 static int ka_launch(const KaArgs& a, cudaStream_t st) {
-  constexpr int bytes = ka_smem_bytes<R>(NG);
+  constexpr int bytes = ka_smem_bytes<ka_warps(NG), R>(NG);
   static std::atomic<bool> attr[kMaxDevices];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -696,8 +800,8 @@ static int ka_launch(const KaArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return set_cuda_error(e, "kv4 attention: cudaFuncSetAttribute");
     attr[dev].store(true, std::memory_order_release);
   }
-  const int ctas = ka_ctas(R);
-  kv4_attn_kernel<NG, R><<<ctas, KA_THREADS, bytes, st>>>(a);
+  const int ctas = ka_ctas(KV4_D / NG);
+  kv4_attn_kernel<NG, R><<<ctas, ka_warps(NG) * 32, bytes, st>>>(a);
   launched();
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "kv4 attention launch");
@@ -728,7 +832,7 @@ uint64_t ltxb_attention_kv4_workspace_bytes(const ltxb_kv4_cache* cache, int row
   c.rows = rows;
   uint64_t bytes;
   if (kv4_use_tc(c, H / c.heads, &bytes, &t)) return bytes;
-  return ka_workspace(ka_rows(rows, c.batch, H / c.heads));
+  return ka_workspace(ka_rows(rows, c.batch, H / c.heads), cache->group);
 }
 
 int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, const void* q, int64_t ldq, void* out,
@@ -749,7 +853,7 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
   uint64_t need = 0;
   Kv4Tc t{};
   const bool tc = kv4_use_tc(a.c, a.G, &need, &t);
-  if (!tc) need = ka_workspace(R);
+  if (!tc) need = ka_workspace(R, cache->group);
   if (!workspace || workspace_bytes < need)
     return set_error(LTXB_EINVAL, "kv4 attention: workspace of %llu bytes is smaller than the %llu required",
                      (unsigned long long)workspace_bytes, (unsigned long long)need);
@@ -768,7 +872,7 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
     return kv4_attention_tc(a.c, t, gate, out, a.causal, st);
   }
   a.cut = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)ka_ctas(R) * 16);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)ka_ctas(cache->group) * 16);
   const int ng = KV4_D / cache->group;
   if (R == 8) {
     if (ng == 1) return ka_launch<1, 8>(a, st);

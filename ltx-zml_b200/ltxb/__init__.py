@@ -216,6 +216,23 @@ def _device(dev):
     return _HERE_NOW if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
+def _stream_on(stream, dev) -> int:
+    """The stream's handle, or that of `dev`'s current one (torch.cuda.current_stream
+    builds an object first: 3 us of a call that may take 5)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index) if stream is None else stream.cuda_stream
+
+
+def _scratch(nbytes: int, dev, stream):
+    """Workspace of one call. It goes back to the allocator when the call has
+    returned, so a stream that is not the current one is made known to it."""
+    if not nbytes:
+        return None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    if stream is not None:
+        t.record_stream(stream)
+    return t
+
+
 def _stream(stream) -> int:
     s = stream if stream is not None else torch.cuda.current_stream()
     return s.cuda_stream
@@ -928,7 +945,7 @@ class KV4Cache:
 
     def _call(self, fn, stream, *args) -> None:
         with _device(self.device):
-            _check(fn(self._ref, *args, _stream(stream)))
+            _check(fn(self._ref, *args, _stream_on(stream, self.device)))
 
     def append(self, k, v, row_start=None, stream=None) -> None:
         """Quantise k, v [rows, kv_heads, 128] bf16 (rows may be strided) into the sequences' last tokens."""
@@ -945,7 +962,8 @@ class KV4Cache:
         if dtype not in (torch.bfloat16, torch.float32):
             raise LtxbError(EINVAL, "read: dtype must be bfloat16 or float32")
         if out is None:
-            out = tuple(torch.empty(rows, self.kv_heads, 128, dtype=dtype, device=self.device) for _ in range(2))
+            both = torch.empty(2, rows, self.kv_heads, 128, dtype=dtype, device=self.device)
+            out = both[0], both[1]
         for t in out:
             if t.dtype != dtype or tuple(t.shape) != (rows, self.kv_heads, 128) or t.device != self.device:
                 raise LtxbError(EINVAL, f"read: outputs must be {dtype} [{rows}, {self.kv_heads}, 128] on {self.device}")
@@ -960,19 +978,22 @@ def attention_kv4(q, cache: KV4Cache, row_start=None, causal: bool = True, gate=
     """softmax(q k^T * scale) v over each sequence's 4-bit cache; q [rows, H,
     128] bf16 (rows may be strided), H a multiple of the cache's heads, the
     rows a sequence's last tokens. gate: f32 [rows, H] or None."""
-    rows, H, hd = q.shape
+    rows, H, _ = q.shape
     ldq = _row_tensor(q, H, "q", cache.device)
-    out = torch.empty(rows, H, hd, dtype=torch.bfloat16, device=q.device) if out is None else out
-    if out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != q.device:
+    if out is None:
+        out = torch.empty(rows, H, 128, dtype=torch.bfloat16, device=cache.device)
+    elif out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != cache.device:
         raise LtxbError(EINVAL, "out must be bf16 like q")
     if gate is not None and (gate.dtype != torch.float32 or tuple(gate.shape) != (rows, H) or gate.device != q.device):
         raise LtxbError(EINVAL, f"gate must be f32 [{rows}, {H}] on {q.device}")
     rs = _index_tensor(row_start, (cache.batch + 1,), "row_start", cache.device)
     if workspace is None:
-        need = int(lib.ltxb_attention_kv4_workspace_bytes(cache._ref, rows, H))
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        with _device(cache.device):  # its size goes by the device's number of SMs
+            need = lib.ltxb_attention_kv4_workspace_bytes(cache._ref, rows, H)
+        workspace = _scratch(need, cache.device, stream)
+    ws, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel())
     cache._call(lib.ltxb_attention_kv4, stream, rs, q.data_ptr(), ldq, _ptr(out), _ptr(gate), rows, H, int(causal),
-                1.0 / np.sqrt(hd) if scale is None else float(scale), _ptr(workspace), workspace.numel())
+                128 ** -0.5 if scale is None else float(scale), ws, ws_bytes)
     return out
 
 
@@ -1030,18 +1051,19 @@ def dq4_gemm(a, wq, scales, bias=None, out=None, workspace=None, stream=None) ->
         raise LtxbError(EINVAL, "dq4_gemm: a bf16 [M, K], wq uint8 [N, K / 2], scales f32 or bf16 [N, K / group]")
     if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,)):
         raise LtxbError(EINVAL, f"dq4_gemm: bias must be bf16 [{N}]")
-    out = torch.empty((M, N), dtype=torch.bfloat16, device=dev) if out is None else out
-    if out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
+    if out is None:
+        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
         raise LtxbError(EINVAL, f"dq4_gemm: out must be bf16 [{M}, {N}]")
-    if any(t is not None and t.device != dev for t in (wq, scales, bias, out, workspace)):
-        raise LtxbError(EINVAL, "dq4_gemm: tensors on different devices")
+    for t in (wq, scales, bias, out, workspace):
+        if t is not None and t.device != dev:
+            raise LtxbError(EINVAL, "dq4_gemm: tensors on different devices")
     if workspace is None:
-        need = int(lib.ltxb_dq4_gemm_workspace_bytes(M, N, K))
-        workspace = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        workspace = _scratch(lib.ltxb_dq4_gemm_workspace_bytes(M, N, K), dev, stream)
     with _device(dev):
         _check(lib.ltxb_dq4_gemm(_ptr(a), _ptr(wq), _ptr(scales), DT_BF16 if scales.dtype == torch.bfloat16 else DT_F32,
                                  K // scales.shape[1], _ptr(bias), _ptr(out), M, N, K, _ptr(workspace),
-                                 0 if workspace is None else workspace.numel(), _stream(stream)))
+                                 0 if workspace is None else workspace.numel(), _stream_on(stream, dev)))
     return out
 
 
