@@ -1,35 +1,41 @@
 // Attention of a few query rows over the paged 4-bit K/V cache (decoding and
 // short runs of tokens): softmax(q k^T * scale) v with k, v = zero + scale_kv * code.
 //
-// The codes go to the tensor cores with almost no arithmetic. K: a code put
-// into the mantissa of an f16 reads u = 1 + c / 16 (mantissa bits 6-9) or
-// 1 + c / 256 (bits 2-5); q's values at the second kind of place are held 16
-// times larger, and the accumulator starts from -sum q (1 + 8 / 16 or
-// 1 + 8 / 256), so one shift and two logic operations unpack four codes and
-//   q . (z + s c) = 16 s acc + (z + 8 s) sum q,  acc = sum q (c - 8) / 16.
-// V: the sum over tokens is long, so its codes enter without an offset:
+// The codes go to the tensor cores with little arithmetic. K: the bytes 0 .. 15
+// are integers, so a mask and a shift unpack eight codes into two operand
+// registers of the 32-deep integer MMA, and
+//   q . (z + s c) = s acc + z sum q,  acc = sum q c.
+// q enters as a 16-bit integer per row (two signed bytes: 256 hi + lo), the
+// row's largest value being 32512, so a value is off by at most 2^-16 of it:
+// scores of typical rows move by some 1e-5. The integer sums start from the
+// bits of 1.5 * 2^23, which makes the accumulators f32 numbers without a
+// conversion. (e4m3 operands, in which a byte 0 .. 15 is code * 2^-9, gave the
+// same sums but ran as f16 with conversions here: 169 us against 117 at
+// 131,009 tokens x 32 heads.)
+// V: p needs more range and bits than e4m3 has, so the codes enter as f16:
 // 1024 + c and 1024 + 16 c (mantissa bits 0-3 and 4-7) are taken to c - 8 by
 // one FMA each, exactly, and
 //   sum_t p_t (z + s c) = sum (p s) (c - 8) + sum p (z + 8 s).
 // Scale and zero thus touch only score-sized data (per group of 32 / 64 / 128).
 //
-// A warp takes 16 tokens of a page as the M side of mma.m16n8k16, so up to 8
-// query rows (the query heads that share the K/V head, times the call's
-// tokens) cost the same as one: S^T = K Q^T, then O^T = V^T P^T with P^T
-// transposed in registers (movmatrix). q enters as f16 after a power of two
-// per row (its 8 bits stay exact down to 2^-27 of the row's largest value).
-// p s enters as f16 scaled by a power of two that follows the largest V scale
-// seen (between 2^3 and 2^7 times p): 11 significant bits where bf16 would
-// keep 8, so the result's own rounding dominates. Row maxima move only when a
-// score passes them by 2^8; sums and accumulators are f32.
+// A warp takes 16 tokens of a page as the M side of the MMA, so up to 8 query
+// rows (the query heads that share the K/V head, times the call's tokens)
+// cost the same as one: S^T = K Q^T, then O^T = V^T P^T with P^T transposed in
+// registers (movmatrix). p s enters as f16 scaled by a power of two that
+// follows the largest V scale seen (between 2^3 and 2^7 times p): 11
+// significant bits where bf16 would keep 8, so the result's own rounding
+// dominates. Row maxima move only when a score passes them by 2^8; sums and
+// accumulators are f32.
 //
 // Work is split by pages, not by sequence: all (sequence, head, row tile)
 // items laid end to end are one line of pages, each CTA takes an equal piece
 // of it, its warps take the pages of an item in turn, and a second kernel
 // joins the items that were cut (in page order, so results do not depend on
-// timing). Lengths are read on the device only. A warp has two slots of one
-// (page, head) block each, filled by one bulk copy (8.5 - 10 KB) while it
-// works on the other: no barrier between warps until an item ends.
+// timing). Lengths are read on the device only. A warp has room for one
+// (page, head) block of its own: the next page's K (codes and pairs, two bulk
+// copies) arrives while it works on V, the next V while it works on K, and no
+// barrier joins the warps until an item ends. 16 warps an SM (12 with groups
+// of 32, or 16 rows) keep about 70 KB per SM in flight.
 //
 // A token whose V group is stored as NaN, or whose page number is bad, makes
 // every row that attends to it NaN and no others: where a page holds tokens
@@ -42,6 +48,8 @@
 
 namespace ltxb {
 
+constexpr float kMagic = 12582912.f;      // 1.5 * 2^23: bits kMagicBits + n are the f32 number kMagic + n, |n| < 2^22
+constexpr int kMagicBits = 0x4B400000;
 constexpr int KA_OLD = KV4_D + 4;  // floats per row of the warps' O tiles
 
 struct KaArgs {
@@ -70,6 +78,19 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// unsigned x signed bytes, 32 deep; d = a b + c
+__device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
+}
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -81,10 +102,6 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// K: from w << 2 (PART 0: nibbles 0, 4 and 1, 5) or w >> 6 (PART 1: nibbles 2,
-// 6 and 3, 7) the f16 pairs 1 + c / 256 (LO) or 1 + c / 16
-__device__ __forceinline__ uint32_t code_lo(uint32_t s) { return (s & 0x003C003Cu) | 0x3C003C00u; }
-__device__ __forceinline__ uint32_t code_hi(uint32_t s) { return (s & 0x03C003C0u) | 0x3C003C00u; }
 // V: the f16 pair c - 8 from bits 0-3 / 4-7 of both halves
 __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
@@ -169,39 +186,45 @@ __device__ __forceinline__ bool ka_next(const KaArgs& a, KaSeg& k) {
   return true;
 }
 
-template <int NW, int R>
+constexpr int KA_WARPS = 4, KA_THREADS = KA_WARPS * 32;
+template <int R>
 struct KaSmem {
-  uint64_t full[NW][2];
-  int good[NW][2];  // the slot's page number was valid
-  long long scan[NW];
+  float o[KA_WARPS][R][KA_OLD];  // the warps' O tiles, joined when an item ends
+  float m[KA_WARPS][R], l[KA_WARPS][R];
+  uint64_t kfull[KA_WARPS], vfull[KA_WARPS];
+  int good[KA_WARPS][2];  // the page number was valid (of even and odd pages)
+  // the CTA's item and each warp's loading place: here and not in registers,
+  // which the accumulators need
+  KaSeg at;
+  KaSeg ls[KA_WARPS];
+  int lp[KA_WARPS];
+  const uint8_t* src[KA_WARPS];  // the block whose V is still to be fetched; null: a bad page
+  long long scan[KA_WARPS];
   int found[4];
-  int busy[NW];     // the warp had pages of the item
-  float m[NW][R], l[NW][R];
 };
-template <int NW, int R>
+template <int R>
 constexpr int ka_smem_bytes(int ng) {
-  return NW * 2 * kv4_block(ng) + (int)sizeof(KaSmem<NW, R>) + 128;
+  return KA_WARPS * kv4_block(ng) + (int)sizeof(KaSmem<R>) + 128;
 }
-// Warps a CTA and CTAs an SM: as many warps as find two slots each in an
-// SM's 227 KB (12 of 8.5 or 9 KB, 10 of 10 KB).
-__host__ __device__ constexpr int ka_warps(int ng) { return ng == 4 ? 5 : 4; }
-__host__ __device__ constexpr int ka_per_sm(int ng) { return ng == 4 ? 2 : 3; }
+// CTAs an SM: four take 128 registers a thread and 52 KB each; 16 rows need
+// more registers, groups of 32 more of both.
+__host__ __device__ constexpr int ka_per_sm(int ng, int R) { return 3; }
 
 template <int NG, int R>
-__global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_kernel(const KaArgs a) {
-  constexpr int NT = R / 8, BLK = kv4_block(NG), NW = ka_warps(NG), THREADS = NW * 32;
-  constexpr int MT = NG * NT <= 1 ? 4 : 2;  // tiles of 16 tokens whose scores are held at once
+__global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(const KaArgs a) {
+  constexpr int NT = R / 8, BLK = kv4_block(NG), NW = KA_WARPS, THREADS = KA_THREADS;
+  constexpr int MT = R == 8 ? 4 : 2;        // tiles of 16 tokens whose scores are held at once
+  constexpr int PAIRS = KV4_PAGE * 4 * NG;  // bytes of a page's K or V pairs
   extern __shared__ __align__(128) uint8_t ka_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ka_raw) + 127) & ~uintptr_t(127));
-  KaSmem<NW, R>& sm = *reinterpret_cast<KaSmem<NW, R>*>(ring + NW * 2 * BLK);
-  static_assert(R * KA_OLD * 4 <= BLK, "a warp's O tile takes the place of a block");
+  KaSmem<R>& sm = *reinterpret_cast<KaSmem<R>*>(ring + NW * BLK);
   const int tid = threadIdx.x, warp = warp_id(), lane = lane_id(), g = lane >> 2, cq = lane & 3;
   const int Hq = a.c.heads * a.G;
 
   if (tid == 0) {
     for (int i = 0; i < NW; ++i) {
-      mbar_init(&sm.full[i][0], 1);
-      mbar_init(&sm.full[i][1], 1);
+      mbar_init(&sm.kfull[i], 1);
+      mbar_init(&sm.vfull[i], 1);
     }
     fence_mbar_init();
     sm.found[0] = -1;
@@ -222,7 +245,9 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
   long long total = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) total += sm.scan[w];
-  const int ctas = total < gridDim.x ? (int)total : (int)gridDim.x;
+  // at least a page for every warp of a CTA
+  const long long most = (total + NW - 1) / NW;
+  const int ctas = most < gridDim.x ? (int)most : (int)gridDim.x;
   // sequences without tokens: their rows attend to nothing and are zero
   for (int b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
     int first, count;
@@ -237,7 +262,6 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
     return;
   }
   const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-  KaSeg at;
   {  // the sequence that holds u0: prefix sums over THREADS sequences at a time
     long long base = 0;
     for (int b0 = 0;; b0 += THREADS) {
@@ -272,81 +296,116 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
       if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
       return;
     }
-    at.b = sm.found[0];
-    at.rt = sm.found[1];
-    at.h = sm.found[2];
-    at.pa = sm.found[3];
-    at.left = u1 - u0;
-    ka_seq<R>(a, at);
-    ka_end(at);
+    if (tid < NW) {
+      KaSeg k;
+      k.b = sm.found[0];
+      k.rt = sm.found[1];
+      k.h = sm.found[2];
+      k.pa = sm.found[3];
+      k.left = u1 - u0;
+      ka_seq<R>(a, k);
+      ka_end(k);
+      sm.ls[tid] = k;
+      sm.lp[tid] = k.pa + tid;
+      if (tid == 0) sm.at = k;
+    }
+    __syncthreads();
   }
 
-  // ---- loads: this warp's pages in order, alternately into its two slots (lane 0) ----
-  uint8_t* slots = ring + warp * 2 * BLK;
-  KaSeg ls = at;
-  int lp = at.pa + warp, sent = 0;
-  bool more = true;
-  auto send = [&]() {
-    while (more && lp >= ls.pb) {
-      more = ka_next<R>(a, ls);
+  // ---- loads (lane 0): this warp's pages in order; K of the next page, then its V ----
+  uint8_t* sk = ring + warp * BLK;       // K codes, K pairs
+  uint8_t* sv = sk + KV4_VOFF + PAIRS;   // V codes, V pairs
+  int sent = 0;
+  auto send_k = [&]() {
+    KaSeg& ls = sm.ls[warp];
+    int lp = sm.lp[warp];
+    while (lp >= ls.pb) {
+      if (ls.left <= 0 || !ka_next<R>(a, ls)) return;
       lp = ls.pa + warp;
     }
-    if (!more) return;
-    const int p = kv4_page(a.c, ls.b, lp), st = sent & 1;
-    sm.good[warp][st] = p >= 0;
-    if (p >= 0) {
-      mbar_arrive_expect_tx(&sm.full[warp][st], BLK);
-      bulk_load(slots + st * BLK, kv4_block_at(a.c, p, ls.h, BLK), BLK, &sm.full[warp][st]);
+    const int p = kv4_page(a.c, ls.b, lp);
+    sm.good[warp][sent & 1] = p >= 0;
+    const uint8_t* src = p >= 0 ? kv4_block_at(a.c, p, ls.h, BLK) : nullptr;
+    if (src) {
+      mbar_arrive_expect_tx(&sm.kfull[warp], KV4_VOFF + PAIRS);
+      bulk_load(sk, src, KV4_VOFF, &sm.kfull[warp]);
+      bulk_load(sk + KV4_VOFF, src + KV4_KPAIR, PAIRS, &sm.kfull[warp]);
     } else {
-      mbar_arrive(&sm.full[warp][st]);
+      mbar_arrive(&sm.kfull[warp]);
     }
+    sm.src[warp] = src;
+    sm.lp[warp] = lp + NW;
     ++sent;
-    lp += NW;
+  };
+  auto send_v = [&]() {
+    const uint8_t* src = sm.src[warp];
+    if (src) {
+      mbar_arrive_expect_tx(&sm.vfull[warp], KV4_VOFF + PAIRS);
+      bulk_load(sv, src + KV4_VOFF, KV4_VOFF, &sm.vfull[warp]);
+      bulk_load(sv + KV4_VOFF, src + kv4_vpair(NG), PAIRS, &sm.vfull[warp]);
+    } else {
+      mbar_arrive(&sm.vfull[warp]);
+    }
   };
   if (lane == 0) {
-    send();
-    send();
+    send_k();
+    if (sent > 0) send_v();
   }
   __syncwarp();
 
   bool ok = true, failed = false, go = true;
-  int used = 0;  // pages this warp has taken from its slots
+  int used = 0;  // pages this warp has done
   while (go) {
-    // ---- a new item: its query rows as f16, sums of q, nothing accumulated ----
-    uint32_t qf[NT][16];
-    uint64_t qs[NT][NG], rs[NT];      // rows 2 c, 2 c + 1: sum q per group; softmax scale * log2(e) / the row's power
-    float init[NT][NG][2];            // -sum q (1 + 8 / 16 or 1 + 8 / 256)
+    const KaSeg& at = sm.at;
+    // ---- a new item: its query rows as two bytes a value, sums of q, nothing accumulated ----
+    uint32_t qf[NT][16];  // [j][hi, lo][even dims, odd dims of the lane's eight]
+    uint64_t qs[NT][NG], rs[NT], l[NT], zs[NT][NG];  // rows 2 c, 2 c + 1: sum q; softmax scale * log2(e) * the row's unit; ...
     float o[NT][8][4], m[NT][2];
-    uint64_t l[NT], zs[NT][NG];
     int lim[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = at.rt * R + t * 8 + g, tok = r / a.G;
       const bool has = tok < at.count;
-      const __nv_bfloat16* src =
+      const __nv_bfloat16* qp =
           a.q + (size_t)(at.first + (has ? tok : 0)) * a.ldq + (at.h * a.G + (has ? r - tok * a.G : 0)) * KV4_D + 8 * cq;
       uint4 w[4];
       float top = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        w[j] = has ? __ldg(reinterpret_cast<const uint4*>(src + 32 * j)) : make_uint4(0, 0, 0, 0);
+        w[j] = has ? __ldg(reinterpret_cast<const uint4*>(qp + 32 * j)) : make_uint4(0, 0, 0, 0);
         const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) top = fmaxf(top, fmaxf(fabsf(bf16_lo(ws[i])), fabsf(bf16_hi(ws[i]))));
+        for (int i = 0; i < 4; ++i) {
+          const float x = fabsf(bf16_lo(ws[i])), y = fabsf(bf16_hi(ws[i]));
+          top = !(x < INFINITY) || !(y < INFINITY) ? NAN : top == top ? fmaxf(top, fmaxf(x, y)) : top;
+        }
       }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      int field = 264 - (int)(__float_as_uint(top) >> 23);  // the largest value into [2^10, 2^11)
-      field = field < 1 ? 1 : field > 249 ? 249 : field;
-      const float f = __uint_as_float((uint32_t)field << 23), f16 = 16.f * f;
+#pragma unroll
+      for (int i = 1; i < 4; i <<= 1) {
+        const float y = __shfl_xor_sync(0xffffffffu, top, i);
+        top = top != top || y != y ? NAN : fmaxf(top, y);
+      }
+      const float pre = top < 8.7e-19f ? 7.378697629483821e19f : 1.f;  // 2^66: the quotient stays in f32's range
+      const float f = top > 0.f ? 32512.f / (top * pre) : 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        qf[t][4 * j + 0] = pack_f16x2(bf16_lo(w[j].x) * f16, bf16_lo(w[j].z) * f16);  // dims 0, 4 of the eight
-        qf[t][4 * j + 1] = pack_f16x2(bf16_hi(w[j].x) * f, bf16_hi(w[j].z) * f);      // 1, 5
-        qf[t][4 * j + 2] = pack_f16x2(bf16_lo(w[j].y) * f16, bf16_lo(w[j].w) * f16);  // 2, 6
-        qf[t][4 * j + 3] = pack_f16x2(bf16_hi(w[j].y) * f, bf16_hi(w[j].w) * f);      // 3, 7
+        const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+        uint32_t byte[2][2] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {  // dims 2 i + y
+            const int v = __float2int_rn((y ? bf16_hi(ws[i]) : bf16_lo(ws[i])) * pre * f);
+            const int hi = (v + 128) >> 8;
+            byte[0][y] |= (uint32_t)(hi & 255) << (8 * i);
+            byte[1][y] |= (uint32_t)((v - 256 * hi) & 255) << (8 * i);
+          }
+        qf[t][4 * j] = byte[0][0];
+        qf[t][4 * j + 1] = byte[0][1];
+        qf[t][4 * j + 2] = byte[1][0];
+        qf[t][4 * j + 3] = byte[1][1];
       }
-      const float back = __uint_as_float((uint32_t)(254 - field) << 23) * a.cs;
+      const float back = top * (a.cs / 32512.f);  // NaN for a row that is not finite
       rs[t] = f2(__shfl_sync(0xffffffffu, back, 8 * cq), __shfl_sync(0xffffffffu, back, 8 * cq + 4));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -361,16 +420,16 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
         for (int e = 0; e < 4; ++e) o[t][x][e] = 0.f;
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
-        float s[4] = {0.f, 0.f, 0.f, 0.f}, n[4] = {0.f, 0.f, 0.f, 0.f};
+        int s[2][4] = {};
 #pragma unroll
-        for (int y = 0; y < 8 / NG; ++y) {
-          const int k = x * (8 / NG) + y;
-          mma_f16(s, 0x2C002C00u, 0x2C002C00u, 0x3C003C00u, 0x3C003C00u, qf[t][2 * k], qf[t][2 * k + 1]);
-          mma_f16(n, 0xBC20BC20u, 0xBC20BC20u, 0xBE00BE00u, 0xBE00BE00u, qf[t][2 * k], qf[t][2 * k + 1]);
-        }
-        qs[t][x] = f2(s[0], s[1]);
-        init[t][x][0] = n[0];
-        init[t][x][1] = n[1];
+        for (int y = 0; y < 4 / NG; ++y)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int i = 4 * (x * (4 / NG) + y) + 2 * e;
+            mma_i8(s[e], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, qf[t][i], qf[t][i + 1], s[e][0], s[e][1],
+                   s[e][2], s[e][3]);
+          }
+        qs[t][x] = f2((float)(256 * s[0][0] + s[1][0]), (float)(256 * s[0][1] + s[1][1]));
         zs[t][x] = 0;
       }
     }
@@ -379,61 +438,55 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
     float sig = 1.f, sig_max = 0.f;  // p s is held as p * (s * sig); sig moves when s passes sig_max
     const int npg = at.pb - at.pa > warp ? (at.pb - at.pa - warp + NW - 1) / NW : 0;
     for (int k = 0; k < npg; ++k, ++used) {
-      const int st = used & 1;
-      if (ok) ok = warp_wait(&sm.full[warp][st], (used >> 1) & 1, 0x301);
+      if (ok) ok = warp_wait(&sm.kfull[warp], used & 1, 0x301);
       if (!ok) break;
-      const uint8_t* blk = slots + st * BLK;
-      const int page = at.pa + warp + k * NW;
-      const bool good = sm.good[warp][st] != 0;
-      const bool whole = good && page * KV4_PAGE + KV4_PAGE - 1 <= all;
+      const int page0 = (at.pa + warp + k * NW) * KV4_PAGE;
+      const bool good = sm.good[warp][used & 1] != 0;
+      const bool whole = good && page0 + KV4_PAGE - 1 <= all;
 #pragma unroll 1
       for (int h = 0; h < 4 / MT; ++h) {
+        // ---- S^T: MT tiles of 16 tokens x R rows; a lane has tokens g, g + 8, rows 2 c, 2 c + 1 ----
         uint64_t s[MT][NT][2];
-        float svm = 0.f;
-        const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + kv4_vpair(NG)) + (h * MT * 16 + g) * NG;
-        // ---- S^T of MT tiles: 16 tokens x R rows each, lane: tokens g, g + 8, rows 2 c, 2 c + 1 ----
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           const int t0 = (h * MT + mt) * 16 + g;
-          const uint4 k0 = *reinterpret_cast<const uint4*>(blk + t0 * 64 + cq * 16);
-          const uint4 k1 = *reinterpret_cast<const uint4*>(blk + (t0 + 8) * 64 + cq * 16);
+          const uint4 k0 = *reinterpret_cast<const uint4*>(sk + t0 * 64 + cq * 16);
+          const uint4 k1 = *reinterpret_cast<const uint4*>(sk + (t0 + 8) * 64 + cq * 16);
           const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-          float acc[NT][NG][4];
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int x = 0; x < NG; ++x) {
-              acc[t][x][0] = acc[t][x][2] = init[t][x][0];
-              acc[t][x][1] = acc[t][x][3] = init[t][x][1];
-            }
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int x = j * NG / 4;
-            const uint32_t a0 = w0[j] << 2, a1 = w1[j] << 2, b0 = w0[j] >> 6, b1 = w1[j] >> 6;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              mma_f16(acc[t][x], code_lo(a0), code_lo(a1), code_hi(a0), code_hi(a1), qf[t][4 * j], qf[t][4 * j + 1]);
-              mma_f16(acc[t][x], code_lo(b0), code_lo(b1), code_hi(b0), code_hi(b1), qf[t][4 * j + 2], qf[t][4 * j + 3]);
-            }
-          }
-          const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + KV4_KPAIR) + t0 * NG;
+          const uint32_t* kp = reinterpret_cast<const uint32_t*>(sk + KV4_VOFF) + t0 * NG;
 #pragma unroll
           for (int x = 0; x < NG; ++x) {
-            const uint32_t p0 = kp[x], p1 = kp[8 * NG + x];
-            const float s0 = bf16_lo(p0), s1 = bf16_lo(p1);
-            const float z0 = fmaf(8.f, s0, bf16_hi(p0)), z1 = fmaf(8.f, s1, bf16_hi(p1));
-            const float a0 = 16.f * s0, a1 = 16.f * s1;
+            int acc[NT][2][4];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              uint64_t y0 = f2mul(f2(z0, z0), qs[t][x]), y1 = f2mul(f2(z1, z1), qs[t][x]);
-              if (x > 0) {
-                y0 = f2add(y0, s[mt][t][0]);
-                y1 = f2add(y1, s[mt][t][1]);
-              }
-              s[mt][t][0] = f2fma(f2(a0, a0), f2(acc[t][x][0], acc[t][x][1]), y0);
-              s[mt][t][1] = f2fma(f2(a1, a1), f2(acc[t][x][2], acc[t][x][3]), y1);
+            for (int y = 0; y < 4 / NG; ++y) {
+              const int j = x * (4 / NG) + y;
+              const uint32_t a0 = w0[j] & 0x0F0F0F0Fu, a1 = w1[j] & 0x0F0F0F0Fu;                // dims 0, 2, 4, 6 of the eight
+              const uint32_t a2 = (w0[j] >> 4) & 0x0F0F0F0Fu, a3 = (w1[j] >> 4) & 0x0F0F0F0Fu;  // 1, 3, 5, 7
+#pragma unroll
+              for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                  int(&d)[4] = acc[t][e];
+                  const uint32_t b0 = qf[t][4 * j + 2 * e], b1 = qf[t][4 * j + 2 * e + 1];
+                  if (y == 0)
+                    mma_i8(d, a0, a1, a2, a3, b0, b1, kMagicBits, kMagicBits, kMagicBits, kMagicBits);
+                  else
+                    mma_i8(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
+                }
             }
-            svm = fmaxf(svm, fmaxf(bf16_lo(vp[mt * 16 * NG + x]), bf16_lo(vp[(mt * 16 + 8) * NG + x])));
+            const uint32_t p0 = kp[x], p1 = kp[8 * NG + x];
+            const float s0 = bf16_lo(p0), s1 = bf16_lo(p1), z0 = bf16_hi(p0), z1 = bf16_hi(p1);
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const uint64_t nm = f2(-kMagic, -kMagic);
+                const uint64_t hi = f2add(f2(__int_as_float(acc[t][0][2 * y]), __int_as_float(acc[t][0][2 * y + 1])), nm);
+                const uint64_t lo = f2add(f2(__int_as_float(acc[t][1][2 * y]), __int_as_float(acc[t][1][2 * y + 1])), nm);
+                const float sy = y ? s1 : s0, zy = y ? z1 : z0;
+                const uint64_t zq = x ? f2fma(f2(zy, zy), qs[t][x], s[mt][t][y]) : f2mul(f2(zy, zy), qs[t][x]);
+                s[mt][t][y] = f2fma(f2(sy, sy), f2fma(hi, f2(256.f, 256.f), lo), zq);
+              }
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -441,21 +494,31 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
             s[mt][t][1] = f2mul(s[mt][t][1], rs[t]);
           }
         }
-        // ---- a page that holds tokens some row does not see ----
-        if (!whole) {
+        __syncwarp();
+        if (lane == 0 && (h + 1) * MT == 4) send_k();  // the next page's (its V follows when this page's has been read)
+        __syncwarp();
+        if (h == 0) ok = warp_wait(&sm.vfull[warp], used & 1, 0x302);
+        if (!ok) break;
+        const uint32_t* vp = reinterpret_cast<const uint32_t*>(sv + KV4_VOFF) + (h * MT * 16 + g) * NG;
+        float svm;
+        if (whole) {  // the largest scale: positive bf16 values order like their bits
+          uint32_t x = 0;
+#pragma unroll
+          for (int i = 0; i < 2 * MT * NG; ++i) x = __vmaxu2(x, vp[(i / NG) * 8 * NG + i % NG]);
+          svm = bf16_lo(x);
+        } else {  // a page that holds tokens some row does not see
           svm = 0.f;
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
-              const int key = page * KV4_PAGE + (h * MT + mt) * 16 + y * 8 + g;
+              const int key = page0 + (h * MT + mt) * 16 + y * 8 + g;
               float bad = good ? 0.f : NAN;  // NaN for a row that sees a token which is not finite
               const bool in = key < at.len && good;
 #pragma unroll
               for (int x = 0; x < NG; ++x) {
                 const uint32_t p = vp[(mt * 16 + y * 8) * NG + x];
-                const float z = fmaf(8.f, bf16_lo(p), bf16_hi(p));
-                if (!(fabsf(z) < INFINITY))
+                if (!(fabsf(fmaf(8.f, bf16_lo(p), bf16_hi(p))) < INFINITY))
                   bad = NAN;
                 else if (in)
                   svm = fmaxf(svm, bf16_lo(p));
@@ -480,8 +543,8 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
             float x0, x1, x2, x3;
             un2(s[mt][t][0], x0, x1);
             un2(s[mt][t][1], x2, x3);
-            top[t][0] = mt ? fmaxf(top[t][0], fmaxf(x0, x2)) : fmaxf(x0, x2);
-            top[t][1] = mt ? fmaxf(top[t][1], fmaxf(x1, x3)) : fmaxf(x1, x3);
+            top[t][0] = mt ? fmax3(top[t][0], x0, x2) : fmaxf(x0, x2);
+            top[t][1] = mt ? fmax3(top[t][1], x1, x3) : fmaxf(x1, x3);
           }
           move = move || top[t][0] > m[t][0] + 8.f || top[t][1] > m[t][1] + 8.f;
         }
@@ -540,12 +603,12 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const uint32_t p = vp[(mt * 16 + y * 8) * NG + x];
-              float sv = bf16_lo(p), zv = fmaf(8.f, sv, bf16_hi(p));
+              float sc = bf16_lo(p), zv = fmaf(8.f, sc, bf16_hi(p));
               if (!whole) {
-                const int key = page * KV4_PAGE + (h * MT + mt) * 16 + y * 8 + g;
-                if (key >= at.len || !good || !(fabsf(zv) < INFINITY)) sv = zv = 0.f;
+                const int key = page0 + (h * MT + mt) * 16 + y * 8 + g;
+                if (key >= at.len || !good || !(fabsf(zv) < INFINITY)) sc = zv = 0.f;
               }
-              const float f = sv * sig;
+              const float f = sc * sig;
 #pragma unroll
               for (int t = 0; t < NT; ++t) {
                 zs[t][x] = f2fma(p2[t][y], f2(zv, zv), zs[t][x]);
@@ -554,7 +617,7 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
                 pb[t][x][y] = transpose8x8(pack_f16x2(x0, x1));
               }
             }
-          const uint8_t* vb = blk + KV4_VOFF + (h * MT + mt) * 1024 + lane * 16;
+          const uint8_t* vb = sv + (h * MT + mt) * 1024 + lane * 16;
           const uint4 v0 = *reinterpret_cast<const uint4*>(vb), v1 = *reinterpret_cast<const uint4*>(vb + 512);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
@@ -572,13 +635,13 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
           }
         }
       }
+      if (!ok) break;
       __syncwarp();
-      if (lane == 0 && k + 1 < npg) send();  // the last page's slot serves as this warp's O tile first
+      if (lane == 0 && sent > used + 1) send_v();
       __syncwarp();
     }
     // ---- the item, or this CTA's piece of it, is done: join the warps ----
-    float* ot = reinterpret_cast<float*>(slots + ((used - 1) & 1) * BLK);  // with pages only: the slot just read
-    if (ok && npg > 0) {
+    if (ok) {
       const float back = 1.f / sig;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -605,14 +668,13 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float zz = z[j * NG / 4][e];
-            *reinterpret_cast<float4*>(ot + r * KA_OLD + 32 * j + 4 * g) =
+            *reinterpret_cast<float4*>(&sm.o[warp][r][32 * j + 4 * g]) =
                 make_float4(fmaf(o[t][2 * j][e], back, zz), fmaf(o[t][2 * j][2 + e], back, zz),
                             fmaf(o[t][2 * j + 1][e], back, zz), fmaf(o[t][2 * j + 1][2 + e], back, zz));
           }
         }
       }
     }
-    if (lane == 0) sm.busy[warp] = npg > 0 ? 1 + ((used - 1) & 1) : 0;  // 1 + the slot that holds the O tile
     failed = __syncthreads_or(!ok);
     if (failed) break;
     const bool ends = at.pb == at.pages, whole_item = ends && at.pa == 0;
@@ -621,23 +683,19 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
     for (int r = warp; r < R; r += NW) {
       const int rr = at.rt * R + r, tok = rr / a.G, head = at.h * a.G + (rr - tok * a.G);
       if (tok >= at.count) break;
-      float top = -FLT_MAX;
-#pragma unroll
-      for (int w = 0; w < NW; ++w)
-        if (sm.busy[w]) top = fmaxf(top, sm.m[w][r]);
+      const float top = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
       float sum = 0.f;
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < NW; ++w)
-        if (sm.busy[w]) {
-          const float f = ka_ex2(sm.m[w][r] - top);
-          const float4 x = *reinterpret_cast<const float4*>(ring + (w * 2 + sm.busy[w] - 1) * BLK + (r * KA_OLD + 4 * lane) * 4);
-          sum = fmaf(sm.l[w][r], f, sum);
-          v.x = fmaf(x.x, f, v.x);
-          v.y = fmaf(x.y, f, v.y);
-          v.z = fmaf(x.z, f, v.z);
-          v.w = fmaf(x.w, f, v.w);
-        }
+      for (int w = 0; w < NW; ++w) {
+        const float f = ka_ex2(sm.m[w][r] - top);
+        const float4 x = *reinterpret_cast<const float4*>(&sm.o[w][r][4 * lane]);
+        sum = fmaf(sm.l[w][r], f, sum);
+        v.x = fmaf(x.x, f, v.x);
+        v.y = fmaf(x.y, f, v.y);
+        v.z = fmaf(x.z, f, v.z);
+        v.w = fmaf(x.w, f, v.w);
+      }
       if (whole_item) {
         const size_t orow = (size_t)(at.first + tok) * Hq + head;
         const float f = (sum == 0.f ? 0.f : 1.f / sum) * (a.gate ? __ldg(a.gate + orow) : 1.f);
@@ -651,11 +709,15 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
         }
       }
     }
-    const KaSeg was = at;
-    go = ka_next<R>(a, at);
-    if (!go && tid == 0) {
+    __syncthreads();  // the O tiles and the item have been read
+    if (tid == 0) {
+      const KaSeg was = sm.at;
+      KaSeg k = was;
+      const bool next = ka_next<R>(a, k);
+      sm.at = k;
+      sm.found[0] = next;
       int4 cut = make_int4(-1, 0, 0, 0);
-      if (was.pa == 0 && !ends) {
+      if (!next && was.pa == 0 && was.pb != was.pages) {
         // the item's last page on the line of pages, and the CTA that has it
         const long long end = u1 - 1 + (was.pages - was.pb);
         long long z = (end * ctas) / total;
@@ -663,21 +725,20 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
         while (total * z / ctas > end) --z;
         cut = make_int4(was.b, was.rt, was.h, (int)z);
       }
-      a.cut[blockIdx.x] = cut;
+      if (!next) a.cut[blockIdx.x] = cut;
     }
-    fence_proxy_async_smem();  // the O tiles were written and read as ordinary memory; copies follow
     __syncthreads();
-    if (lane == 0 && npg > 0) send();
-    __syncwarp();
+    go = sm.found[0] != 0;
   }
   // a failed wait (reported in the status word) leaves copies under way: let
   // them land before this CTA's shared memory is given up
   if (failed) {
-    if (lane == 0) {
+    if (lane == 0 && sent > used) {
       const uint64_t t0 = globaltimer_ns();
-      for (int i = used; i < sent; ++i)
-        while (!mbar_try_wait(smem_u32(&sm.full[warp][i & 1]), (i >> 1) & 1) && globaltimer_ns() - t0 < kWaitLimitNs) {
-        }
+      while ((!mbar_try_wait(smem_u32(&sm.kfull[warp]), (sent - 1) & 1) ||
+              !mbar_try_wait(smem_u32(&sm.vfull[warp]), used & 1)) &&
+             globaltimer_ns() - t0 < kWaitLimitNs) {
+      }
     }
     if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
   }
@@ -685,13 +746,13 @@ __global__ void __launch_bounds__(ka_warps(NG) * 32, ka_per_sm(NG)) kv4_attn_ker
 
 // Joins the pieces of the items that were cut: CTA (x, y) takes row y of the
 // item that starts in attention CTA x and goes on to CTA cut[x].w. Its pieces
-// are slot 2 x + 1 and slots 2 i, i = x + 1 .. w, taken in that order by four
+// are slot 2 x + 1 and slots 2 i, i = x + 1 .. w, taken in that order by eight
 // warps in turn, whose sums are added in warp order.
 template <int R>
-__global__ void __launch_bounds__(128) kv4_join_kernel(const KaArgs a) {
+__global__ void __launch_bounds__(256) kv4_join_kernel(const KaArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  __shared__ float sm_m[4], sm_l[4];
-  __shared__ float4 sm_o[4][32];
+  __shared__ float sm_m[8], sm_l[8];
+  __shared__ float4 sm_o[8][32];
   const int4 cut = a.cut[blockIdx.x];
   if (cut.x < 0) return;
   const int warp = warp_id(), lane = lane_id(), r = blockIdx.y;
@@ -703,16 +764,17 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const KaArgs a) {
   constexpr int SLOT = R * (KV4_D + 2);
   auto slot = [&](int i) { return a.part + (size_t)(2 * (blockIdx.x + i) + (i == 0 ? 1 : 0)) * SLOT; };
   float top = -FLT_MAX;
-  for (int i = threadIdx.x; i < pieces; i += 128) top = fmaxf(top, slot(i)[R * KV4_D + r]);
+  for (int i = threadIdx.x; i < pieces; i += 256) top = fmaxf(top, slot(i)[R * KV4_D + r]);
 #pragma unroll
   for (int k = 1; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
   if (lane == 0) sm_m[warp] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(sm_m[0], sm_m[1]), fmaxf(sm_m[2], sm_m[3]));
+#pragma unroll
+  for (int w = 0; w < 8; ++w) top = fmaxf(top, sm_m[w]);
   float sum = 0.f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-  for (int i = warp; i < pieces; i += 4) {
+  for (int i = warp; i < pieces; i += 8) {
     const float* s = slot(i);
     const float f = ka_ex2(s[R * KV4_D + r] - top);
     const float4 x = *reinterpret_cast<const float4*>(s + r * KV4_D + 4 * lane);
@@ -726,13 +788,19 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const KaArgs a) {
   if (lane == 0) sm_l[warp] = sum;
   __syncthreads();
   if (warp == 0) {
-    sum = (sm_l[0] + sm_l[1]) + (sm_l[2] + sm_l[3]);
-    const float4 x0 = sm_o[0][lane], x1 = sm_o[1][lane], x2 = sm_o[2][lane], x3 = sm_o[3][lane];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) {
+      const float4 x = sm_o[w][lane];
+      sum += sm_l[w];
+      v.x += x.x;
+      v.y += x.y;
+      v.z += x.z;
+      v.w += x.w;
+    }
     const size_t orow = (size_t)(first + tok) * a.c.heads * a.G + cut.z * a.G + (rr - tok * a.G);
     const float f = (sum == 0.f ? 0.f : 1.f / sum) * (a.gate ? __ldg(a.gate + orow) : 1.f);
     *reinterpret_cast<uint2*>(a.out + orow * KV4_D + 4 * lane) =
-        make_uint2(pack_bf16x2(((x0.x + x1.x) + (x2.x + x3.x)) * f, ((x0.y + x1.y) + (x2.y + x3.y)) * f),
-                   pack_bf16x2(((x0.z + x1.z) + (x2.z + x3.z)) * f, ((x0.w + x1.w) + (x2.w + x3.w)) * f));
+        make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
   }
 }
 
@@ -782,15 +850,15 @@ static bool kv4_use_tc(const Kv4View& c, int G, uint64_t* bytes, Kv4Tc* t) {
 // Query rows of a tile: 8 where every sequence's rows fit (one n8 tile of
 // the MMA), else 16, which unpacks a page once for twice the rows.
 static int ka_rows(int rows, int batch, int G) { return (int64_t)rows * G <= 8ll * batch ? 8 : 16; }
-static int ka_ctas(int group) { return sm_count() * ka_per_sm(KV4_D / group); }
+static int ka_ctas(int R, int group) { return sm_count() * ka_per_sm(KV4_D / group, R); }
 static uint64_t ka_workspace(int R, int group) {
-  const uint64_t n = ka_ctas(group);
+  const uint64_t n = ka_ctas(R, group);
   return n * 16 + n * 2 * R * (KV4_D + 2) * 4;
 }
 
 template <int NG, int R>
 static int ka_launch(const KaArgs& a, cudaStream_t st) {
-  constexpr int bytes = ka_smem_bytes<ka_warps(NG), R>(NG);
+  constexpr int bytes = ka_smem_bytes<R>(NG);
   static std::atomic<bool> attr[kMaxDevices];
   int dev = 0;
   cudaGetDevice(&dev);
@@ -800,14 +868,14 @@ static int ka_launch(const KaArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return set_cuda_error(e, "kv4 attention: cudaFuncSetAttribute");
     attr[dev].store(true, std::memory_order_release);
   }
-  const int ctas = ka_ctas(KV4_D / NG);
-  kv4_attn_kernel<NG, R><<<ctas, ka_warps(NG) * 32, bytes, st>>>(a);
+  const int ctas = ka_ctas(R, KV4_D / NG);
+  kv4_attn_kernel<NG, R><<<ctas, KA_THREADS, bytes, st>>>(a);
   launched();
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e, "kv4 attention launch");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(ctas, R);
-  cfg.blockDim = dim3(128);
+  cfg.blockDim = dim3(256);
   cfg.stream = st;
   cudaLaunchAttribute la[1];
   la[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -872,7 +940,7 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
     return kv4_attention_tc(a.c, t, gate, out, a.causal, st);
   }
   a.cut = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)ka_ctas(cache->group) * 16);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)ka_ctas(R, cache->group) * 16);
   const int ng = KV4_D / cache->group;
   if (R == 8) {
     if (ng == 1) return ka_launch<1, 8>(a, st);
