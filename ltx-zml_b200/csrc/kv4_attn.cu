@@ -1,27 +1,25 @@
 // Attention of a few query rows over the paged 4-bit K/V cache (decoding and
 // short runs of tokens): softmax(q k^T * scale) v with k, v = zero + scale_kv * code.
 //
-// The codes go to the tensor cores with little arithmetic. K: the bytes 0 .. 15
-// are integers, so a mask and a shift unpack eight codes into two operand
-// registers of the 32-deep integer MMA, and
-//   q . (z + s c) = s acc + z sum q,  acc = sum q c.
-// q enters as a 16-bit integer per row (two signed bytes: 256 hi + lo), the
-// row's largest value being 32512, so a value is off by at most 2^-16 of it:
-// scores of typical rows move by some 1e-5. The integer sums start from the
-// bits of 1.5 * 2^23, which makes the accumulators f32 numbers without a
-// conversion. (e4m3 operands, in which a byte 0 .. 15 is code * 2^-9, gave the
-// same sums but ran as f16 with conversions here: 169 us against 117 at
-// 131,009 tokens x 32 heads.)
-// V: p needs more range and bits than e4m3 has, so the codes enter as f16:
-// 1024 + c and 1024 + 16 c (mantissa bits 0-3 and 4-7) are taken to c - 8 by
-// one FMA each, exactly, and
-//   sum_t p_t (z + s c) = sum (p s) (c - 8) + sum p (z + 8 s).
+// The codes go to the tensor cores as they are: a nibble alone in the lowest
+// mantissa bits of an f16 is the subnormal code * 2^-24, in the next four bits
+// code * 2^-20, both exact and without an offset, so one shift and four masks
+// unpack eight codes into four operand registers of mma.m16n8k16, and
+//   q . (z + s c)       = s sum q c + z sum q
+//   sum_t p_t (z + s c) = sum (p s) c + sum p z.
+// K: q's values at the first kind of place are held 16 times larger, so that
+// both kinds add up in units of 2^-20. V: the two kinds are rows of their own.
+// (Other forms that were measured at 131,009 tokens x 32 heads: 1 + c / 16 with
+// the offset taken out by one more MMA, 205 us with 16 tokens a step; c - 8 by
+// an f16 FMA a pair, 149; K through the integer MMA with q in two bytes, 136;
+// K as e4m3, which runs as f16 with conversions here, 169.)
 // Scale and zero thus touch only score-sized data (per group of 32 / 64 / 128).
 //
 // A warp takes 16 tokens of a page as the M side of the MMA, so up to 8 query
 // rows (the query heads that share the K/V head, times the call's tokens)
 // cost the same as one: S^T = K Q^T, then O^T = V^T P^T with P^T transposed in
-// registers (movmatrix). p s enters as f16 scaled by a power of two that
+// registers (movmatrix). q enters as f16 after a power of two per row (its 8
+// bits stay exact down to 2^-27 of the row's largest value). p s enters as f16 scaled by a power of two that
 // follows the largest V scale seen (between 2^3 and 2^7 times p): 11
 // significant bits where bf16 would keep 8, so the result's own rounding
 // dominates. Row maxima move only when a score passes them by 2^8; sums and
@@ -48,8 +46,6 @@
 
 namespace ltxb {
 
-constexpr float kMagic = 12582912.f;      // 1.5 * 2^23: bits kMagicBits + n are the f32 number kMagic + n, |n| < 2^22
-constexpr int kMagicBits = 0x4B400000;
 constexpr int KA_OLD = KV4_D + 4;  // floats per row of the warps' O tiles
 
 struct KaArgs {
@@ -78,14 +74,6 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// unsigned x signed bytes, 32 deep; d = a b + c
-__device__ __forceinline__ void mma_i8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-      : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c0), "r"(c1), "r"(c2), "r"(c3));
-}
 __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -102,18 +90,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// V: the f16 pair c - 8 from bits 0-3 / 4-7 of both halves
-__device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ uint32_t code_0(uint32_t w) {  // (1024 + c) - 1032
-  return h2_fma((w & 0x000F000Fu) | 0x64006400u, 0x3C003C00u, 0xE408E408u);
-}
-__device__ __forceinline__ uint32_t code_1(uint32_t w) {  // (1024 + 16 c) / 16 - 72
-  return h2_fma((w & 0x00F000F0u) | 0x64006400u, 0x2C002C00u, 0xD480D480u);
-}
+// f16 pairs code * 2^-24 (bits 0-3 of both halves) and code * 2^-20 (bits 4-7)
+__device__ __forceinline__ uint32_t code_0(uint32_t w) { return w & 0x000F000Fu; }
+__device__ __forceinline__ uint32_t code_1(uint32_t w) { return w & 0x00F000F0u; }
 // two-wide f32
 __device__ __forceinline__ uint64_t f2(float a, float b) {
   uint64_t r;
@@ -198,7 +177,6 @@ struct KaSmem {
   KaSeg at;
   KaSeg ls[KA_WARPS];
   int lp[KA_WARPS];
-  const uint8_t* src[KA_WARPS];  // the block whose V is still to be fetched; null: a bad page
   long long scan[KA_WARPS];
   int found[4];
 };
@@ -208,7 +186,7 @@ constexpr int ka_smem_bytes(int ng) {
 }
 // CTAs an SM: four take 128 registers a thread and 52 KB each; 16 rows need
 // more registers, groups of 32 more of both.
-__host__ __device__ constexpr int ka_per_sm(int ng, int R) { return 3; }
+__host__ __device__ constexpr int ka_per_sm(int ng, int R) { return ng == 4 || R == 16 ? 3 : 4; }
 
 template <int NG, int R>
 __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(const KaArgs a) {
@@ -315,30 +293,40 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
   // ---- loads (lane 0): this warp's pages in order; K of the next page, then its V ----
   uint8_t* sk = ring + warp * BLK;       // K codes, K pairs
   uint8_t* sv = sk + KV4_VOFF + PAIRS;   // V codes, V pairs
-  int sent = 0;
-  auto send_k = [&]() {
+  int sent = 0, np = -1;         // np: the number of the next page (its table entry is fetched a page ahead)
+  bool more = true;
+  const uint8_t* src = nullptr;  // the block whose V is still to be fetched; null: a bad page
+  auto find = [&]() {            // the next page of this warp
     KaSeg& ls = sm.ls[warp];
     int lp = sm.lp[warp];
     while (lp >= ls.pb) {
-      if (ls.left <= 0 || !ka_next<R>(a, ls)) return;
+      if (!ka_next<R>(a, ls)) {
+        more = false;
+        return;
+      }
       lp = ls.pa + warp;
     }
-    const int p = kv4_page(a.c, ls.b, lp);
-    sm.good[warp][sent & 1] = p >= 0;
-    const uint8_t* src = p >= 0 ? kv4_block_at(a.c, p, ls.h, BLK) : nullptr;
-    if (src) {
+    sm.lp[warp] = lp + NW;
+    const size_t i = (size_t)ls.b * a.c.max_pages + lp;
+    np = a.c.table ? __ldg(a.c.table + i) : (int)i;
+  };
+  auto send_k = [&]() {
+    if (!more) return;
+    const bool good = (unsigned)np < (unsigned)a.c.n_pages;
+    src = good ? kv4_block_at(a.c, np, sm.ls[warp].h, BLK) : nullptr;
+    sm.good[warp][sent & 1] = good;
+    if (good) {
       mbar_arrive_expect_tx(&sm.kfull[warp], KV4_VOFF + PAIRS);
       bulk_load(sk, src, KV4_VOFF, &sm.kfull[warp]);
       bulk_load(sk + KV4_VOFF, src + KV4_KPAIR, PAIRS, &sm.kfull[warp]);
     } else {
+      report_index(LTXB_SITE_KV4_PAGE);
       mbar_arrive(&sm.kfull[warp]);
     }
-    sm.src[warp] = src;
-    sm.lp[warp] = lp + NW;
     ++sent;
+    find();
   };
   auto send_v = [&]() {
-    const uint8_t* src = sm.src[warp];
     if (src) {
       mbar_arrive_expect_tx(&sm.vfull[warp], KV4_VOFF + PAIRS);
       bulk_load(sv, src + KV4_VOFF, KV4_VOFF, &sm.vfull[warp]);
@@ -348,6 +336,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
     }
   };
   if (lane == 0) {
+    find();
     send_k();
     if (sent > 0) send_v();
   }
@@ -357,8 +346,8 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
   int used = 0;  // pages this warp has done
   while (go) {
     const KaSeg& at = sm.at;
-    // ---- a new item: its query rows as two bytes a value, sums of q, nothing accumulated ----
-    uint32_t qf[NT][16];  // [j][hi, lo][even dims, odd dims of the lane's eight]
+    // ---- a new item: its query rows as f16, sums of q, nothing accumulated ----
+    uint32_t qf[NT][16];  // [j][nibbles 0 4, 1 5, 2 6, 3 7 of the lane's word]
     uint64_t qs[NT][NG], rs[NT], l[NT], zs[NT][NG];  // rows 2 c, 2 c + 1: sum q; softmax scale * log2(e) * the row's unit; ...
     float o[NT][8][4], m[NT][2];
     int lim[NT][2];
@@ -385,27 +374,17 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
         const float y = __shfl_xor_sync(0xffffffffu, top, i);
         top = top != top || y != y ? NAN : fmaxf(top, y);
       }
-      const float pre = top < 8.7e-19f ? 7.378697629483821e19f : 1.f;  // 2^66: the quotient stays in f32's range
-      const float f = top > 0.f ? 32512.f / (top * pre) : 0.f;
+      int field = 264 - (int)((__float_as_uint(top) >> 23) & 255u);  // the largest value into [2^10, 2^11)
+      field = field < 1 ? 1 : field > 249 ? 249 : field;
+      const float f = __uint_as_float((uint32_t)field << 23), f16 = 16.f * f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t ws[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-        uint32_t byte[2][2] = {};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {  // dims 2 i + y
-            const int v = __float2int_rn((y ? bf16_hi(ws[i]) : bf16_lo(ws[i])) * pre * f);
-            const int hi = (v + 128) >> 8;
-            byte[0][y] |= (uint32_t)(hi & 255) << (8 * i);
-            byte[1][y] |= (uint32_t)((v - 256 * hi) & 255) << (8 * i);
-          }
-        qf[t][4 * j] = byte[0][0];
-        qf[t][4 * j + 1] = byte[0][1];
-        qf[t][4 * j + 2] = byte[1][0];
-        qf[t][4 * j + 3] = byte[1][1];
+        qf[t][4 * j + 0] = pack_f16x2(bf16_lo(w[j].x) * f16, bf16_lo(w[j].z) * f16);  // dims 0, 4 of the eight
+        qf[t][4 * j + 1] = pack_f16x2(bf16_hi(w[j].x) * f, bf16_hi(w[j].z) * f);      // 1, 5
+        qf[t][4 * j + 2] = pack_f16x2(bf16_lo(w[j].y) * f16, bf16_lo(w[j].w) * f16);  // 2, 6
+        qf[t][4 * j + 3] = pack_f16x2(bf16_hi(w[j].y) * f, bf16_hi(w[j].w) * f);      // 3, 7
       }
-      const float back = top * (a.cs / 32512.f);  // NaN for a row that is not finite
+      const float back = top == top ? __uint_as_float((uint32_t)(254 - field) << 23) * a.cs : NAN;  // not finite: a NaN row
       rs[t] = f2(__shfl_sync(0xffffffffu, back, 8 * cq), __shfl_sync(0xffffffffu, back, 8 * cq + 4));
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -420,16 +399,13 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
         for (int e = 0; e < 4; ++e) o[t][x][e] = 0.f;
 #pragma unroll
       for (int x = 0; x < NG; ++x) {
-        int s[2][4] = {};
+        float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int y = 0; y < 4 / NG; ++y)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int i = 4 * (x * (4 / NG) + y) + 2 * e;
-            mma_i8(s[e], 0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u, qf[t][i], qf[t][i + 1], s[e][0], s[e][1],
-                   s[e][2], s[e][3]);
-          }
-        qs[t][x] = f2((float)(256 * s[0][0] + s[1][0]), (float)(256 * s[0][1] + s[1][1]));
+        for (int y = 0; y < 8 / NG; ++y) {  // rows of 1/16 and 1
+          const int i = 2 * (x * (8 / NG) + y);
+          mma_f16(s, 0x2C002C00u, 0x2C002C00u, 0x3C003C00u, 0x3C003C00u, qf[t][i], qf[t][i + 1]);
+        }
+        qs[t][x] = f2(s[0], s[1]);
         zs[t][x] = 0;
       }
     }
@@ -456,37 +432,28 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
           const uint32_t* kp = reinterpret_cast<const uint32_t*>(sk + KV4_VOFF) + t0 * NG;
 #pragma unroll
           for (int x = 0; x < NG; ++x) {
-            int acc[NT][2][4];
+            float acc[NT][4];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
 #pragma unroll
             for (int y = 0; y < 4 / NG; ++y) {
               const int j = x * (4 / NG) + y;
-              const uint32_t a0 = w0[j] & 0x0F0F0F0Fu, a1 = w1[j] & 0x0F0F0F0Fu;                // dims 0, 2, 4, 6 of the eight
-              const uint32_t a2 = (w0[j] >> 4) & 0x0F0F0F0Fu, a3 = (w1[j] >> 4) & 0x0F0F0F0Fu;  // 1, 3, 5, 7
+              const uint32_t a0 = w0[j], a1 = w1[j], b0 = w0[j] >> 8, b1 = w1[j] >> 8;
 #pragma unroll
-              for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  int(&d)[4] = acc[t][e];
-                  const uint32_t b0 = qf[t][4 * j + 2 * e], b1 = qf[t][4 * j + 2 * e + 1];
-                  if (y == 0)
-                    mma_i8(d, a0, a1, a2, a3, b0, b1, kMagicBits, kMagicBits, kMagicBits, kMagicBits);
-                  else
-                    mma_i8(d, a0, a1, a2, a3, b0, b1, d[0], d[1], d[2], d[3]);
-                }
+              for (int t = 0; t < NT; ++t) {
+                mma_f16(acc[t], code_0(a0), code_0(a1), code_1(a0), code_1(a1), qf[t][4 * j], qf[t][4 * j + 1]);
+                mma_f16(acc[t], code_0(b0), code_0(b1), code_1(b0), code_1(b1), qf[t][4 * j + 2], qf[t][4 * j + 3]);
+              }
             }
             const uint32_t p0 = kp[x], p1 = kp[8 * NG + x];
-            const float s0 = bf16_lo(p0), s1 = bf16_lo(p1), z0 = bf16_hi(p0), z1 = bf16_hi(p1);
+            const float s0 = 1048576.f * bf16_lo(p0), s1 = 1048576.f * bf16_lo(p1), z0 = bf16_hi(p0), z1 = bf16_hi(p1);
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int y = 0; y < 2; ++y) {
-                const uint64_t nm = f2(-kMagic, -kMagic);
-                const uint64_t hi = f2add(f2(__int_as_float(acc[t][0][2 * y]), __int_as_float(acc[t][0][2 * y + 1])), nm);
-                const uint64_t lo = f2add(f2(__int_as_float(acc[t][1][2 * y]), __int_as_float(acc[t][1][2 * y + 1])), nm);
-                const float sy = y ? s1 : s0, zy = y ? z1 : z0;
-                const uint64_t zq = x ? f2fma(f2(zy, zy), qs[t][x], s[mt][t][y]) : f2mul(f2(zy, zy), qs[t][x]);
-                s[mt][t][y] = f2fma(f2(sy, sy), f2fma(hi, f2(256.f, 256.f), lo), zq);
-              }
+            for (int t = 0; t < NT; ++t) {
+              const uint64_t y0 = x ? f2fma(f2(z0, z0), qs[t][x], s[mt][t][0]) : f2mul(f2(z0, z0), qs[t][x]);
+              const uint64_t y1 = x ? f2fma(f2(z1, z1), qs[t][x], s[mt][t][1]) : f2mul(f2(z1, z1), qs[t][x]);
+              s[mt][t][0] = f2fma(f2(s0, s0), f2(acc[t][0], acc[t][1]), y0);
+              s[mt][t][1] = f2fma(f2(s1, s1), f2(acc[t][2], acc[t][3]), y1);
+            }
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -518,7 +485,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
 #pragma unroll
               for (int x = 0; x < NG; ++x) {
                 const uint32_t p = vp[(mt * 16 + y * 8) * NG + x];
-                if (!(fabsf(fmaf(8.f, bf16_lo(p), bf16_hi(p))) < INFINITY))
+                if (!(fabsf(bf16_lo(p) + bf16_hi(p)) < INFINITY))
                   bad = NAN;
                 else if (in)
                   svm = fmaxf(svm, bf16_lo(p));
@@ -603,10 +570,10 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const uint32_t p = vp[(mt * 16 + y * 8) * NG + x];
-              float sc = bf16_lo(p), zv = fmaf(8.f, sc, bf16_hi(p));
+              float sc = bf16_lo(p), zv = bf16_hi(p);
               if (!whole) {
                 const int key = page0 + (h * MT + mt) * 16 + y * 8 + g;
-                if (key >= at.len || !good || !(fabsf(zv) < INFINITY)) sc = zv = 0.f;
+                if (key >= at.len || !good || !(fabsf(sc + zv) < INFINITY)) sc = zv = 0.f;
               }
               const float f = sc * sig;
 #pragma unroll
@@ -642,7 +609,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
     }
     // ---- the item, or this CTA's piece of it, is done: join the warps ----
     if (ok) {
-      const float back = 1.f / sig;
+      const float back0 = 16777216.f / sig, back1 = 1048576.f / sig;  // 2^24, 2^20
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float lt[2], z[NG][2];
@@ -659,7 +626,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
           }
           // a NaN group of any V makes the whole row NaN, not its own dims alone
 #pragma unroll
-          for (int x = 0; x < NG; ++x) lt[e] += z[x][e] - z[x][e];
+          for (int x = 0; x < NG; ++x) lt[e] += (z[x][e] - z[x][e]) + (o[t][8 / NG * x][e] - o[t][8 / NG * x][e]);
           const int r = t * 8 + 2 * cq + e;
           if (g == 0) {
             sm.m[warp][r] = m[t][e];
@@ -669,8 +636,8 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
           for (int j = 0; j < 4; ++j) {
             const float zz = z[j * NG / 4][e];
             *reinterpret_cast<float4*>(&sm.o[warp][r][32 * j + 4 * g]) =
-                make_float4(fmaf(o[t][2 * j][e], back, zz), fmaf(o[t][2 * j][2 + e], back, zz),
-                            fmaf(o[t][2 * j + 1][e], back, zz), fmaf(o[t][2 * j + 1][2 + e], back, zz));
+                make_float4(fmaf(o[t][2 * j][e], back0, zz), fmaf(o[t][2 * j][2 + e], back1, zz),
+                            fmaf(o[t][2 * j + 1][e], back0, zz), fmaf(o[t][2 * j + 1][2 + e], back1, zz));
           }
         }
       }
