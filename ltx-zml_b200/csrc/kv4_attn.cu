@@ -186,7 +186,7 @@ constexpr int ka_smem_bytes(int ng) {
 }
 // CTAs an SM: four take 128 registers a thread and 52 KB each; 16 rows need
 // more registers, groups of 32 more of both.
-__host__ __device__ constexpr int ka_per_sm(int ng, int R) { return ng == 4 || R == 16 ? 3 : 4; }
+__host__ __device__ constexpr int ka_per_sm(int ng, int R) { return 3; }
 
 template <int NG, int R>
 __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(const KaArgs a) {
