@@ -3,17 +3,22 @@
 //
 // Quantiser, per token, head and group of 32 / 64 / 128 values x (bf16):
 //   zero = min x, scale = bf16((max x - min x) / 15), code = round((x - zero) / scale),
-// ties to even, code 0 where scale is 0. The code is the one of exact
-// arithmetic: x - zero is rounded once in f32 and multiplied by 1 / scale,
-// and where that product comes within 1e-5 of a half (its error is below
-// 16 * 2^-22 = 4e-6) the quotient is taken again in 64 bits. scale is at
-// least range / 15 * (1 - 2^-8), so the product stays below 15.06 and needs
-// no clamp there.
+// the differences in f32, the quotients exact, ties to even, code 0 where scale
+// is 0. A quotient is a product with 1 / scale and one Newton step: exact where
+// it is a half (ties are common, both sides having few bits) and within 5e-7
+// elsewhere, where no quotient of an f32 difference below 15.06 scales by an
+// 8-bit scale comes closer to a half than 9e-7. scale is at least
+// range / 15 * (1 - 2^-8), so the quotient stays below 15.06: no clamp.
 // A group that holds a NaN or an infinity (or whose range is above the
 // largest f32) stores scale = NaN and reads back as NaN.
 //
 // Both kernels are bandwidth-bound: 512 bytes of bf16 K and V on one side
-// and 128 + 8 NG bytes on the other per token and head.
+// and 128 + 8 NG bytes on the other per token and head. A warp takes the
+// call's tokens of one octet (8 positions, the unit of the V layout) of one
+// head: 4 KB of K and V rows are under way at once, the codes are put in order
+// in shared memory and stored 16 bytes a lane. With one warp per token (4-byte
+// stores into 8 sectors for V) writing and reading back 28,160 tokens x 32
+// heads took 620 us.
 #include "kv4.cuh"
 
 namespace ltxb {
@@ -36,123 +41,225 @@ __device__ __forceinline__ uint32_t bmax2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Four codes (a lane's dims 4 L .. 4 L + 3, nibble i = value i) and the
-// group's (scale, zero) pair of the 4 bf16 values in `w`; the 8 * (4 / NG)
-// lanes of a group agree.
+// The tokens that unit u of the call covers: octet `o` (positions 8 o ..) of
+// sequence b, of which [p0, p1) belong to the call and are row `row0` on; false
+// if there are none. Sequence b's units start at row_start[b] / 8 + 2 b, which
+// leaves room for its octets however its tokens lie in them.
+struct Kv4Octet {
+  int b, p0, p1, row0;
+};
+__device__ __forceinline__ bool kv4_octet(const Kv4View& c, long long u, Kv4Octet* out) {
+  auto start = [&](int b) -> long long {
+    const int r = c.row_start ? __ldg(c.row_start + b) : b * c.per;
+    return (r < 0 ? 0 : r) / 8 + 2ll * b;
+  };
+  int lo = 0, hi = c.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (start(mid) <= u)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  int first, count;
+  kv4_rows(c, lo, &first, &count);
+  const int len = kv4_len(c, lo), begin = len - count;  // position of row `first`; may be negative
+  const int from = begin < 0 ? 0 : begin;
+  const long long o = from / 8 + (u - start(lo));
+  if (u < start(lo) || o * 8 >= len) return false;
+  out->b = lo;
+  out->p0 = (int)(o * 8) < from ? from : (int)(o * 8);
+  out->p1 = (int)(o * 8) + 8 < len ? (int)(o * 8) + 8 : len;
+  out->row0 = first + out->p0 - begin;
+  return true;
+}
+
+// two-wide f32
+__device__ __forceinline__ uint64_t c2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void c2un(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t c2add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t c2mul(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t c2fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// Eight codes (nibble i = value i of a lane's eight consecutive dims) and the
+// group's (scale, zero) pair; the 16 / NG lanes of a group agree.
 template <int NG>
-__device__ __forceinline__ uint32_t kv4_quantise(uint2 w, uint32_t* pair) {
+__device__ __forceinline__ uint32_t kv4_quantise(uint4 v, uint32_t* pair) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   // (max, -min) as one bf16x2: one shuffle and one maximum per step
-  const uint32_t hi = bmax2(w.x, w.y), lo = bmax2(w.x ^ 0x80008000u, w.y ^ 0x80008000u);
+  const uint32_t hi = bmax2(bmax2(w[0], w[1]), bmax2(w[2], w[3]));
+  const uint32_t sign = 0x80008000u;
+  const uint32_t lo = bmax2(bmax2(w[0] ^ sign, w[1] ^ sign), bmax2(w[2] ^ sign, w[3] ^ sign));
   uint32_t mm = bmax2(__byte_perm(hi, lo, 0x5410), __byte_perm(hi, lo, 0x7632));
 #pragma unroll
-  for (int s = 1; s < 32 / NG; s <<= 1) mm = bmax2(mm, __shfl_xor_sync(0xffffffffu, mm, s));
+  for (int s = 1; s < 16 / NG; s <<= 1) mm = bmax2(mm, __shfl_xor_sync(0xffffffffu, mm, s));
   const float top = bf16_lo(mm), zero = -bf16_hi(mm);
   const float range = top - zero;
-  const float q15 = __fdiv_rn(range, 15.0f);
-  const __nv_bfloat16 sb = __float2bfloat16_rn(q15);
+  // range / 15, correctly rounded: product with 1 / 15 and one Newton step
+  const float r15 = range * (1.f / 15.f);
+  const __nv_bfloat16 sb = __float2bfloat16_rn(fmaf(fmaf(-15.f, r15, range), 1.f / 15.f, r15));
   const float scale = __bfloat162float(sb);
   const bool finite = range < INFINITY;  // false for NaN and for infinity
   *pair = finite ? ((mm ^ 0x80000000u) & 0xFFFF0000u) | __bfloat16_as_ushort(sb) : 0x7FFFu;
-  const bool tiny = scale < 7.5e-37f;  // 2^-120: 1 / scale would leave f32's range
-  const float inv = scale > 0.f ? __frcp_rn(scale) : 0.f;
-  const float x[4] = {bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
-  uint32_t code = 0;
-  float far = 0.f;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+  const uint64_t nz = c2(-zero, -zero), in2 = c2(inv, inv), ns = c2(-scale, -scale), mg = c2(12582912.f, 12582912.f),
+                 nm = c2(-12582912.f, -12582912.f);
+  float q[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float t = (x[i] - zero) * inv;
-    const float m = t + 12582912.0f;  // 1.5 * 2^23: the integer in the low mantissa bits
-    far = fmaxf(far, fabsf(t - (m - 12582912.0f)));
-    code |= (__float_as_uint(m) & 15u) << (4 * i);
+    const uint64_t d = c2add(c2(bf16_lo(w[i]), bf16_hi(w[i])), nz), t = c2mul(d, in2);
+    const uint64_t t1 = c2fma(c2fma(ns, t, d), in2, t);
+    c2un(c2add(c2add(t1, mg), nm), q[2 * i], q[2 * i + 1]);  // the nearest integers (1.5 * 2^23 added and taken off)
   }
-  if ((far > 0.49999f || tiny) && scale > 0.f && finite) {
-    code = 0;
+  uint32_t code[2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const double t = rint(((double)x[i] - (double)zero) / (double)scale);
-      code |= (uint32_t)(t > 15.0 ? 15.0 : t) << (4 * i);
-    }
+  for (int h = 0; h < 2; ++h) {  // four codes as one exact number below 2^16, in the low bits of 1.5 * 2^23
+    const float p = fmaf(fmaf(q[4 * h + 3], 16.f, q[4 * h + 2]), 256.f, fmaf(q[4 * h + 1], 16.f, q[4 * h]));
+    code[h] = __float_as_uint(p + 12582912.f);
   }
-  return code;
+  uint32_t out = __byte_perm(code[0], code[1], 0x5410);
+  if (scale < 7.5e-37f || !finite) {  // below 2^-120 1 / scale leaves f32's range: quotients one by one
+    out = 0;
+    if (scale > 0.f && finite)
+#pragma unroll 1
+      for (int i = 0; i < 8; ++i) {
+        const float x = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
+        out |= (uint32_t)fminf(rintf(__fdiv_rn(x - zero, scale)), 15.f) << (4 * i);
+      }
+  }
+  return out;
 }
 
-// One warp per row and head: lane L holds dims 4 L .. 4 L + 3 of K and V.
+// CTA (x, y): octet unit x, heads 8 y + warp. Lane = 16 half + m holds dims
+// 8 m .. 8 m + 7 of tokens 2 i + half, i = 0 .. 3 of the octet.
 template <int NG>
-__global__ void __launch_bounds__(256) kv4_append_kernel(const Kv4View c, const __nv_bfloat16* __restrict__ k,
+__global__ void __launch_bounds__(256, 4) kv4_append_kernel(const Kv4View c, const __nv_bfloat16* __restrict__ k,
                                                          size_t ldk, const __nv_bfloat16* __restrict__ v,
                                                          size_t ldv) {
-  const int lane = lane_id();
-  const long long n = (long long)c.rows * c.heads;
-  for (long long u = blockIdx.x * 8ll + warp_id(); u < n; u += gridDim.x * 8ll) {
-    const int row = (int)(u / c.heads), h = (int)(u % c.heads);
-    const int b = kv4_row_seq(c, row);
-    if (b < 0) continue;
-    int first, count;
-    kv4_rows(c, b, &first, &count);
-    const int pos = kv4_len(c, b) - count + (row - first);
-    if (row < first || row >= first + count || pos < 0) continue;
-    const int page = kv4_page(c, b, pos / KV4_PAGE);
-    if (page < 0) continue;
-    const uint2 kx = *reinterpret_cast<const uint2*>(k + row * ldk + h * KV4_D + lane * 4);
-    const uint2 vx = *reinterpret_cast<const uint2*>(v + row * ldv + h * KV4_D + lane * 4);
+  __shared__ __align__(16) uint8_t codes[8][2][512];
+  const int warp = warp_id(), lane = lane_id(), half = lane >> 4, m = lane & 15;
+  const int h = blockIdx.y * 8 + warp;
+  if (h >= c.heads) return;
+  Kv4Octet oc;
+  if (!kv4_octet(c, blockIdx.x, &oc)) return;
+  const int base = oc.p0 & ~7, t8 = (base % KV4_PAGE) / 8;  // first position, octet of the page
+  const int page = kv4_page(c, oc.b, oc.p0 / KV4_PAGE);     // used after the rows are under way
+  uint4 x[2][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int pos = base + 2 * i + half;
+    const bool in = pos >= oc.p0 && pos < oc.p1;
+    const size_t row = in ? oc.row0 + (pos - oc.p0) : oc.row0;
+    x[0][i] = __ldg(reinterpret_cast<const uint4*>(k + row * ldk + h * KV4_D + 8 * m));
+    x[1][i] = __ldg(reinterpret_cast<const uint4*>(v + row * ldv + h * KV4_D + 8 * m));
+  }
+  if (page < 0) return;
+  uint8_t* blk = const_cast<uint8_t*>(kv4_block_at(c, page, h, kv4_block(NG)));
+  const int j = m >> 2, cc = m & 3;  // dims 32 j + 8 cc .. + 7
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int t = 2 * i + half, pos = base + t;
     uint32_t kp, vp;
-    uint32_t kc = kv4_quantise<NG>(kx, &kp);
-    uint32_t vc = kv4_quantise<NG>(vx, &vp);
-    uint8_t* blk = const_cast<uint8_t*>(kv4_block_at(c, page, h, kv4_block(NG)));
-    const int t = pos % KV4_PAGE;
-    // K: lanes 2 m, 2 m + 1 make one word; V: halves j, j + 1 of chunk g
-    kc |= __shfl_down_sync(0xffffffffu, kc, 1) << 16;
-    vc |= __shfl_down_sync(0xffffffffu, vc, 8) << 16;
-    const int j = lane >> 3, cc = (lane >> 1) & 3, g = lane & 7;
-    if ((lane & 1) == 0) *reinterpret_cast<uint32_t*>(blk + t * 64 + (cc * 4 + j) * 4) = kc;
-    if ((j & 1) == 0)
-      *reinterpret_cast<uint32_t*>(blk + KV4_VOFF + (t >> 3) * 512 + g * 64 + ((t & 7) >> 1) * 16 + (t & 1) * 8 +
-                                   (j >> 1) * 4) = vc;
-    if (lane % (32 / NG) == 0) {
-      const int gi = lane / (32 / NG);
-      *reinterpret_cast<uint32_t*>(blk + KV4_KPAIR + (t * NG + gi) * 4) = kp;
-      *reinterpret_cast<uint32_t*>(blk + kv4_vpair(NG) + (t * NG + gi) * 4) = vp;
+    const uint32_t kc = kv4_quantise<NG>(x[0][i], &kp), vc = kv4_quantise<NG>(x[1][i], &vp);
+    *reinterpret_cast<uint32_t*>(&codes[warp][0][t * 64 + (cc * 4 + j) * 4]) = kc;
+    // halves j of chunks 2 cc and 2 cc + 1
+    uint8_t* vd = &codes[warp][1][2 * cc * 64 + (t >> 1) * 16 + (t & 1) * 8 + j * 2];
+    *reinterpret_cast<uint16_t*>(vd) = (uint16_t)vc;
+    *reinterpret_cast<uint16_t*>(vd + 64) = (uint16_t)(vc >> 16);
+    if (m % (16 / NG) == 0 && pos >= oc.p0 && pos < oc.p1) {
+      const int at = ((t8 * 8 + t) * NG + m / (16 / NG)) * 4;
+      *reinterpret_cast<uint32_t*>(blk + KV4_KPAIR + at) = kp;
+      *reinterpret_cast<uint32_t*>(blk + kv4_vpair(NG) + at) = vp;
     }
   }
+  __syncwarp();
+  const uint4 ko = *reinterpret_cast<const uint4*>(&codes[warp][0][lane * 16]);
+  const uint4 vo = *reinterpret_cast<const uint4*>(&codes[warp][1][lane * 16]);
+  const int kt = base + (lane >> 2), v0 = base + 2 * (lane & 3);  // tokens of the lane's 16 bytes of K; of V, v0 and v0 + 1
+  if (kt >= oc.p0 && kt < oc.p1) *reinterpret_cast<uint4*>(blk + t8 * 512 + lane * 16) = ko;
+  uint8_t* vd = blk + KV4_VOFF + t8 * 512 + lane * 16;
+  const bool in0 = v0 >= oc.p0 && v0 < oc.p1, in1 = v0 + 1 >= oc.p0 && v0 + 1 < oc.p1;
+  if (in0 && in1)
+    *reinterpret_cast<uint4*>(vd) = vo;
+  else if (in0)
+    *reinterpret_cast<uint2*>(vd) = make_uint2(vo.x, vo.y);
+  else if (in1)
+    *reinterpret_cast<uint2*>(vd + 8) = make_uint2(vo.z, vo.w);
 }
 
-// The four values of a lane: zero + scale * code in f32, rounded once.
-__device__ __forceinline__ float4 kv4_values(uint32_t code, uint32_t pair) {
+// Values zero + scale * code in f32, rounded once, of the N = 4 or 8 codes of
+// `code`, stored at `out` (f32 or bf16).
+template <int N, bool F32>
+__device__ __forceinline__ void kv4_values(uint32_t code, uint32_t pair, void* out, size_t at) {
   const float s = bf16_lo(pair), z = bf16_hi(pair);
-  return make_float4(fmaf(s, (float)(code & 15u), z), fmaf(s, (float)((code >> 4) & 15u), z),
-                     fmaf(s, (float)((code >> 8) & 15u), z), fmaf(s, (float)((code >> 12) & 15u), z));
+  const uint64_t s2 = c2(s, s), z2 = c2(z, z), off = c2(-8388608.f, -8388608.f);
+  float f[N];
+#pragma unroll
+  for (int i = 0; i < N; i += 2) {  // 2^23 + code, exactly
+    const uint32_t a = ((code >> (4 * i)) & 15u) | 0x4B000000u, b = ((code >> (4 * i + 4)) & 15u) | 0x4B000000u;
+    c2un(c2fma(s2, c2add(c2(__uint_as_float(a), __uint_as_float(b)), off), z2), f[i], f[i + 1]);
+  }
+  if (F32) {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + at + i) = make_float4(f[i], f[i + 1], f[i + 2], f[i + 3]);
+  } else if (N == 8) {
+    *reinterpret_cast<uint4*>(reinterpret_cast<__nv_bfloat16*>(out) + at) =
+        make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[N - 4], f[N - 3]), pack_bf16x2(f[N - 2], f[N - 1]));
+  } else {
+    *reinterpret_cast<uint2*>(reinterpret_cast<__nv_bfloat16*>(out) + at) = make_uint2(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]));
+  }
 }
 
 template <int NG, bool F32>
 __global__ void __launch_bounds__(256) kv4_read_kernel(const Kv4View c, void* __restrict__ k_out,
                                                        void* __restrict__ v_out) {
-  const int lane = lane_id();
-  const long long n = (long long)c.rows * c.heads;
-  for (long long u = blockIdx.x * 8ll + warp_id(); u < n; u += gridDim.x * 8ll) {
-    const int row = (int)(u / c.heads), h = (int)(u % c.heads);
-    const int b = kv4_row_seq(c, row);
-    if (b < 0) continue;
-    int first, count;
-    kv4_rows(c, b, &first, &count);
-    const int pos = kv4_len(c, b) - count + (row - first);
-    if (row < first || row >= first + count || pos < 0) continue;
-    const int page = kv4_page(c, b, pos / KV4_PAGE);
-    if (page < 0) continue;
-    const uint8_t* blk = kv4_block_at(c, page, h, kv4_block(NG));
-    const int t = pos % KV4_PAGE, j = lane >> 3, cc = (lane >> 1) & 3, g = lane & 7, gi = lane / (32 / NG);
-    const uint32_t kc = *reinterpret_cast<const uint16_t*>(blk + t * 64 + (cc * 4 + j) * 4 + (lane & 1) * 2);
-    const uint32_t vc = *reinterpret_cast<const uint16_t*>(blk + KV4_VOFF + (t >> 3) * 512 + g * 64 +
-                                                           ((t & 7) >> 1) * 16 + (t & 1) * 8 + j * 2);
-    const float4 kf = kv4_values(kc, *reinterpret_cast<const uint32_t*>(blk + KV4_KPAIR + (t * NG + gi) * 4));
-    const float4 vf = kv4_values(vc, *reinterpret_cast<const uint32_t*>(blk + kv4_vpair(NG) + (t * NG + gi) * 4));
-    const size_t o = (size_t)u * 32 + lane;
-    if (F32) {
-      reinterpret_cast<float4*>(k_out)[o] = kf;
-      reinterpret_cast<float4*>(v_out)[o] = vf;
-    } else {
-      reinterpret_cast<uint2*>(k_out)[o] = make_uint2(pack_bf16x2(kf.x, kf.y), pack_bf16x2(kf.z, kf.w));
-      reinterpret_cast<uint2*>(v_out)[o] = make_uint2(pack_bf16x2(vf.x, vf.y), pack_bf16x2(vf.z, vf.w));
-    }
+  const int lane = lane_id(), h = blockIdx.y * 8 + warp_id();
+  if (h >= c.heads) return;
+  Kv4Octet oc;
+  if (!kv4_octet(c, blockIdx.x, &oc)) return;
+  const int page = kv4_page(c, oc.b, oc.p0 / KV4_PAGE);
+  if (page < 0) return;
+  const uint8_t* blk = kv4_block_at(c, page, h, kv4_block(NG));
+  const int base = oc.p0 & ~7, t8 = (base % KV4_PAGE) / 8;
+  const uint4 kw = *reinterpret_cast<const uint4*>(blk + t8 * 512 + lane * 16);
+  const uint4 vw = *reinterpret_cast<const uint4*>(blk + KV4_VOFF + t8 * 512 + lane * 16);
+  const uint32_t* kp = reinterpret_cast<const uint32_t*>(blk + KV4_KPAIR) + t8 * 8 * NG;
+  const uint32_t* vp = reinterpret_cast<const uint32_t*>(blk + kv4_vpair(NG)) + t8 * 8 * NG;
+  const int g = lane >> 2, cq = lane & 3;
+  auto at = [&](int pos) { return ((size_t)(oc.row0 + (pos - oc.p0)) * c.heads + h) * KV4_D; };
+  if (base + g >= oc.p0 && base + g < oc.p1) {
+    const uint32_t w[4] = {kw.x, kw.y, kw.z, kw.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) kv4_values<8, F32>(w[j], kp[g * NG + j * NG / 4], k_out, at(base + g) + 32 * j + 8 * cq);
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int t = 2 * cq + e;
+    if (base + t < oc.p0 || base + t >= oc.p1) continue;
+    const uint32_t w[2] = {e ? vw.z : vw.x, e ? vw.w : vw.y};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      kv4_values<4, F32>(w[j >> 1] >> (16 * (j & 1)), vp[t * NG + j * NG / 4], v_out, at(base + t) + 32 * j + 4 * g);
   }
 }
 
@@ -173,6 +280,7 @@ int kv4_check(const ltxb_kv4_cache* c, const int32_t* row_start, int rows, const
     return set_error(LTXB_EINVAL, "%s: page_table, seq_lens and row_start must be 4-byte aligned", what);
   if (!c->page_table && (int64_t)c->batch * c->max_pages > c->n_pages)
     return set_error(LTXB_EINVAL, "%s: without a page table the cache needs batch * max_pages pages", what);
+  if (c->kv_heads > 65535 * 8 || c->batch > (1 << 28)) return set_error(LTXB_EINVAL, "%s: too many heads or sequences", what);
   if ((int64_t)c->max_pages * KV4_PAGE > INT32_MAX)
     return set_error(LTXB_EINVAL, "%s: sequences of 2^31 tokens or more", what);
   if (rows > 0 && c->batch == 0) return set_error(LTXB_EINVAL, "%s: rows but no sequences", what);
@@ -196,10 +304,8 @@ int kv4_check(const ltxb_kv4_cache* c, const int32_t* row_start, int rows, const
   return LTXB_OK;
 }
 
-static int kv4_grid(const Kv4View& v) {
-  const long long ctas = ((long long)v.rows * v.heads + 7) / 8, most = 8ll * 8 * sm_count();
-  return (int)(ctas < most ? ctas : most);
-}
+// octet units x groups of eight heads
+static dim3 kv4_grid(const Kv4View& v) { return dim3(v.rows / 8 + 2 * v.batch, (v.heads + 7) / 8); }
 
 }  // namespace ltxb
 
@@ -223,7 +329,7 @@ int ltxb_kv4_append(const ltxb_kv4_cache* cache, const int32_t* row_start, const
     return set_error(LTXB_EINVAL, "kv4 append: row strides are smaller than kv_heads * 128");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const __nv_bfloat16 *kb = static_cast<const __nv_bfloat16*>(k), *vb = static_cast<const __nv_bfloat16*>(v);
-  const int grid = kv4_grid(c);
+  const dim3 grid = kv4_grid(c);
   if (cache->group == 128)
     kv4_append_kernel<1><<<grid, 256, 0, st>>>(c, kb, ldk, vb, ldv);
   else if (cache->group == 64)
@@ -245,7 +351,7 @@ int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k
   if (!k_out || !v_out || ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15))
     return set_error(LTXB_EINVAL, "kv4 read: outputs must be 16-byte aligned");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int grid = kv4_grid(c);
+  const dim3 grid = kv4_grid(c);
   auto go = [&](auto kern) { kern<<<grid, 256, 0, st>>>(c, k_out, v_out); };
   const bool f = out_dtype == LTXB_DT_F32;
   if (cache->group == 128)

@@ -24,9 +24,10 @@ def quantise(x: torch.Tensor, group: int):
     """codes [..., 128] int64, scale and zero [..., 128 / group] float64 of bf16-valued x [..., 128]."""
     g = x.double().reshape(*x.shape[:-1], HD // group, group)
     zero = g.amin(-1)
-    rng = g.amax(-1) - zero
+    rng = (g.amax(-1) - zero).float().double()  # the format's differences are those of f32
     scale = bf16(rng / 15)
-    q = torch.where(scale[..., None] > 0, (g - zero[..., None]) / scale[..., None], torch.zeros_like(g))
+    d = (g - zero[..., None]).float().double()
+    q = torch.where(scale[..., None] > 0, d / scale[..., None], torch.zeros_like(g))
     code = torch.round(q).clamp(0, 15)
     bad = ~torch.isfinite(rng)
     scale = torch.where(bad, torch.full_like(scale, math.nan), scale)

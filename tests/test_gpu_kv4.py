@@ -181,7 +181,6 @@ def test_quantiser_at_the_borders(cuda, group):
     cache.append(x.to(cuda), x.to(cuda))
     kf, vf = cache.read(12, dtype=torch.float32)
     want = kr.held(x, group)
-    want[9, 0, :group] = math.nan  # finite in 64 bits; documented as NaN
     for got in (kf.cpu(), vf.cpu()):
         assert torch.equal(got.isnan(), want.isnan())
         assert torch.equal(got.nan_to_num(), want.float().nan_to_num())
