@@ -3,19 +3,27 @@
 // columns of a row, two codes a byte (low half the even column).
 //
 // Few rows (up to DQ4_STREAM_ROWS): bound by the weights' bytes (N K / 2 plus
-// scales). The codes go to the tensor cores as they are: in the top mantissa
-// bits of a bf16 a code c reads u = 1 + c / 16, and
-//   sum x (c - 8) s = 16 s (sum x u - 1.5 sum x)
-// so unpacking costs one shift and one logic operation per two codes, the
-// offset is the accumulator's initial value (one MMA with constant rows
-// -1.5), and the scale is applied once per group to f32 sums. The products
-// are exact; nothing is rounded before the output.
+// scales). The codes go to the tensor cores as they are: a nibble alone in the
+// lowest mantissa bits of an f16 is the subnormal code * 2^-24, in the next
+// four bits code * 2^-20, both exact, so one shift and four masks unpack eight
+// codes into four operand registers of mma.m16n8k16. A's rows enter as f16
+// after a power of two per row and 256 columns (16 times larger where they meet
+// the first kind of nibble; a bf16 value stays exact down to 2^-27 of the
+// largest of the 256), and the accumulator of a group starts from -8 sum x, so
+// that
+//   sum_k x (c - 8) s = s (sum x c - 8 sum x)
+// needs one f32 FMA per group and output. Products are exact, sums f32.
 //
-// A warp takes 16 weight rows as the M side of mma.m16n8k16 and up to 8 NT
-// rows of A as the N side; the warps of a CTA share the 16 rows and split K.
-// Lane 4 g + c loads weight rows g and g + 8, a quarter of each group's
-// columns (16, 8 or 4 bytes for groups of 128, 64, 32), and A's row g at the
-// same columns: both sides of a contraction may be permuted alike.
+// A CTA takes 128 weight rows and 1 / S of K: a producer warp streams
+// [128 rows x 128 bytes] tiles (TMA, 256 columns) through a ring, four warps
+// take 32 rows each (two M tiles, so that a B fragment is read once for both).
+// A's records (its values in the order of the B fragments, the groups' sums)
+// come through the same ring from a kernel of their own, which runs under this
+// one's start; where a CTA has few values of A (DQ4_OWN), its warps make them
+// in shared memory while the ring fills. The S CTAs of a cluster add their f32
+// partials in rank order through distributed shared memory. S fills the SMs
+// where N alone does not: the largest power of two up to 8 that keeps the CTAs
+// within what the SMs hold at once.
 //
 // More rows: the weights are expanded to bf16 in the workspace (one rounding:
 // the code and a bf16 scale have up to 11 significant bits) and multiplied by
@@ -27,50 +35,74 @@
 
 namespace ltxb {
 
-constexpr int DQ4_THREADS = 256, DQ4_WARPS = 8;
 constexpr int DQ4_STREAM_ROWS = 64;
+constexpr int DQ4_WARPS = 8, DQ4_THREADS = 32 * (DQ4_WARPS + 1);
+constexpr int DQ4_OWN = 2048;      // values of A (rows x columns of a CTA) that a CTA puts in order itself
+constexpr int DQ4_OWN_RECORDS = 8; // 2048 columns
+
+// A's record of 256 columns for NT tiles of 8 rows in shared memory: per block
+// of 128 the fragments [tile][word 0 .. 3][lane] of 16 bytes and the
+// accumulators' initial values -8 * 2^-20 * sum x, f32 [group][8 NT]; then
+// 1 / the rows' powers of two, f32 [8 NT].
+__host__ __device__ constexpr int dq4_block(int ng, int nt) { return 2048 * nt + 32 * ng * nt; }
+__host__ __device__ constexpr int dq4_record(int ng, int nt) { return 2 * dq4_block(ng, nt) + 32 * nt; }
 
 struct Dq4Args {
-  const __nv_bfloat16* a;
-  const uint8_t* w;
   const void* scales;
   const __nv_bfloat16* bias;
   __nv_bfloat16* out;
-  int M, N, K, scale_bf16;
+  const __nv_bfloat16* a;
+  const uint8_t* rec;  // [M / (8 NT)][K / 256] records, or null: made from `a` by the CTA
+  int M, N, K, splits;
 };
 
 __device__ __forceinline__ void dq4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// bf16 pair (1 + c / 16) of nibbles I and I + 4 of w
-template <int I>
-__device__ __forceinline__ uint32_t dq4_code(uint32_t w) {
-  const uint32_t s = I == 0 ? w << 3 : w >> (4 * I - 3);
-  return (s & 0x00780078u) | 0x3F803F80u;
+__device__ __forceinline__ uint32_t dq4_pack(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
+__device__ __forceinline__ uint32_t dq4_lo(uint32_t w) { return w & 0x000F000Fu; }
+__device__ __forceinline__ uint32_t dq4_hi(uint32_t w) { return w & 0x00F000F0u; }
 
-// Words y = 0 .. 3 of a lane in a block of 128 columns cover columns
-// dq4_col(y) .. + 7 and lie in group y NG / 4 (NG = 128 / group).
+// Word y = 0 .. 3 of lane quarter c in a block of 128 columns covers columns
+// dq4_col(y, c) .. + 7 and lies in group y NG / 4 (NG = 128 / group): a quad's
+// four words make up 32 columns of one group.
 template <int NG>
 __device__ __forceinline__ int dq4_col(int y, int c) {
   return NG == 1 ? 32 * c + 8 * y : NG == 2 ? 64 * (y >> 1) + 16 * c + 8 * (y & 1) : 32 * y + 8 * c;
 }
-template <int NG>
-__device__ __forceinline__ void dq4_load(const uint8_t* row, int c, uint32_t (&w)[4]) {
-  if (NG == 1) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + 16 * c));
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else if (NG == 2) {
-    const uint2 v0 = __ldg(reinterpret_cast<const uint2*>(row + 8 * c));
-    const uint2 v1 = __ldg(reinterpret_cast<const uint2*>(row + 32 + 8 * c));
-    w[0] = v0.x, w[1] = v0.y, w[2] = v1.x, w[3] = v1.y;
+// The NG scales of one row and block: one aligned load.
+template <int NG, bool BF>
+__device__ __forceinline__ void dq4_scales(const void* s, size_t i, float (&v)[NG]) {
+  if (BF) {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(s) + i * NG;
+    if (NG == 1) {
+      v[0] = __uint_as_float((uint32_t)__ldg(p) << 16);
+    } else if (NG == 2) {
+      const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(p));
+      v[0] = bf16_lo(w), v[NG - 1] = bf16_hi(w);
+    } else {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+      v[0] = bf16_lo(w.x), v[1 % NG] = bf16_hi(w.x), v[2 % NG] = bf16_lo(w.y), v[3 % NG] = bf16_hi(w.y);
+    }
   } else {
-#pragma unroll
-    for (int y = 0; y < 4; ++y) w[y] = __ldg(reinterpret_cast<const uint32_t*>(row + 16 * y + 4 * c));
+    const float* p = reinterpret_cast<const float*>(s) + i * NG;
+    if (NG == 1) {
+      v[0] = __ldg(p);
+    } else if (NG == 2) {
+      const float2 w = __ldg(reinterpret_cast<const float2*>(p));
+      v[0] = w.x, v[NG - 1] = w.y;
+    } else {
+      const float4 w = __ldg(reinterpret_cast<const float4*>(p));
+      v[0] = w.x, v[1 % NG] = w.y, v[2 % NG] = w.z, v[3 % NG] = w.w;
+    }
   }
 }
 __device__ __forceinline__ float dq4_scale(const void* s, int is_bf16, size_t i) {
@@ -78,127 +110,426 @@ __device__ __forceinline__ float dq4_scale(const void* s, int is_bf16, size_t i)
                  : __ldg(reinterpret_cast<const float*>(s) + i);
 }
 
+// One warp: columns [k0, k0 + 256) of the row at `row` (zeros from K on, or
+// everywhere if there is no row) into the record `rec`, as row j of the 8 NT.
 template <int NG, int NT>
-__global__ void __launch_bounds__(DQ4_THREADS) dq4_stream_kernel(const Dq4Args p) {
-  __shared__ float red[DQ4_WARPS][16][8 * NT + 1];
+__device__ __forceinline__ void dq4_put(const __nv_bfloat16* __restrict__ row, int k0, int K, int j, uint8_t* rec) {
+  const int lane = lane_id(), t = j >> 3, g = j & 7;
+  const int k = k0 + 8 * lane;
+  const uint4 v = row && k < K ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  float top = 0.f, s = 0.f;  // the largest finite value; the sum
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = bf16_lo(w[i]), y = bf16_hi(w[i]);
+    if (fabsf(x) < INFINITY) top = fmaxf(top, fabsf(x));
+    if (fabsf(y) < INFINITY) top = fmaxf(top, fabsf(y));
+    s += x + y;
+  }
+#pragma unroll
+  for (int i = 1; i < 32; i <<= 1) {
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    if (i < 16 / NG) s += __shfl_xor_sync(0xffffffffu, s, i);
+  }
+  int field = 264 - (int)(__float_as_uint(top) >> 23);  // the largest value into [2^10, 2^11)
+  field = field < 1 ? 1 : field > 249 ? 249 : field;
+  const float f = __uint_as_float((uint32_t)field << 23), f16 = 16.f * f;
+  // the lane's eight columns are word y of lane quarter c (a quad's four words of one y make up 32 columns of a group)
+  const int q = lane & 15;
+  const int y = NG == 1 ? q & 3 : NG == 2 ? 2 * (q >> 3) + (q & 1) : q >> 2;
+  const int c = NG == 1 ? q >> 2 : NG == 2 ? (q >> 1) & 3 : q & 3;
+  uint8_t* blk = rec + (lane >> 4) * dq4_block(NG, NT);
+  *reinterpret_cast<uint4*>(blk + ((t * 4 + y) * 32 + g * 4 + c) * 16) =
+      make_uint4(dq4_pack(bf16_lo(v.x) * f16, bf16_lo(v.z) * f16), dq4_pack(bf16_hi(v.x) * f, bf16_hi(v.z) * f),
+                 dq4_pack(bf16_lo(v.y) * f16, bf16_lo(v.w) * f16), dq4_pack(bf16_hi(v.y) * f, bf16_hi(v.w) * f));
+  if ((lane & (16 / NG - 1)) == 0)
+    *reinterpret_cast<float*>(blk + 2048 * NT + ((q / (16 / NG)) * 8 * NT + j) * 4) = s * f * -7.62939453125e-06f;
+  if (lane == 0)
+    *reinterpret_cast<float*>(rec + 2 * dq4_block(NG, NT) + j * 4) = __uint_as_float((uint32_t)(254 - field) << 23);
+}
+
+// All records of A, a warp each (row of the 8 NT, 256 columns).
+template <int NG, int NT>
+__global__ void __launch_bounds__(256) dq4_rows_kernel(const __nv_bfloat16* __restrict__ A, int M, int K, int tasks,
+                                                       uint8_t* __restrict__ rec) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int n = (K + 255) / 256;
+  const int x = blockIdx.x * 8 + warp_id();
+  if (x >= tasks) return;
+  const int m = x / n, r = x - m * n, chunk = m / (8 * NT);
+  dq4_put<NG, NT>(m < M ? A + (size_t)m * K : nullptr, r * 256, K, m - chunk * 8 * NT,
+                  rec + ((size_t)chunk * n + r) * dq4_record(NG, NT));
+}
+
+__device__ __forceinline__ void dq4_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+  float v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
+      : "=f"(v)
+      : "r"(addr), "r"(rank)
+      : "memory");
+  return v;
+}
+
+template <int NG, int NT, bool OWN>
+struct Dq4Cfg {
+  static constexpr int ROWS = 128, RT = 1;
+  static constexpr int WBYTES = ROWS * 128, RECORD = dq4_record(NG, NT);
+  static constexpr int STAGE = WBYTES + (OWN ? 0 : (RECORD + 1023) / 1024 * 1024);  // 1 KB: the swizzled tile's alignment
+  static constexpr int PER_SM = 2;
+  static constexpr int STAGES = 4;
+  static constexpr int PART = 8 * NT * (ROWS + 1) * 4;
+  static constexpr int SMEM = STAGES * STAGE + (OWN ? DQ4_OWN_RECORDS * RECORD : 0) + 1024 + 256;
+  static_assert(PART <= STAGES * STAGE, "the partials take the ring's place");
+};
+
+template <int NG, int NT, bool BF, bool OWN>
+__global__ void __launch_bounds__(DQ4_THREADS, Dq4Cfg<NG, NT, OWN>::PER_SM)
+    dq4_stream_kernel(const __grid_constant__ CUtensorMap tmW, const Dq4Args p) {
+  using C = Dq4Cfg<NG, NT, OWN>;
+  constexpr int RT = C::RT;
+  extern __shared__ uint8_t dq4_raw[];
+  uint8_t* ring = dq4_raw + (-smem_u32(dq4_raw) & 1023u);
+  uint8_t* recs = ring + C::STAGES * C::STAGE;  // OWN: this CTA's records
+  uint64_t* full = reinterpret_cast<uint64_t*>(recs + (OWN ? DQ4_OWN_RECORDS * C::RECORD : 0));
+  uint64_t* empty = full + C::STAGES;
   const int warp = warp_id(), lane = lane_id(), g = lane >> 2, c = lane & 3;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 8 * NT;
+  // MMA row g stands for weight row pg of eight: the rows whose words a quarter or
+  // half of a warp loads together then lie in different banks of the swizzled tile
+  const int pg = ((g & 1) << 2) | (g & 2) | (g >> 2);
+  const int n0 = blockIdx.x * C::ROWS, rank = blockIdx.y, S = p.splits;
   const int nkb = p.K / 128;
-  const int kb0 = warp * nkb / DQ4_WARPS, kb1 = (warp + 1) * nkb / DQ4_WARPS;
-  const uint8_t* w0 = p.w + (size_t)(n0 + g) * (p.K / 2);
-  const uint8_t* w1 = w0 + (size_t)8 * (p.K / 2);
-  const size_t s0 = (size_t)(n0 + g) * (nkb * NG), s1 = s0 + (size_t)8 * (nkb * NG);
-  float tot[NT][4];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) tot[t][0] = tot[t][1] = tot[t][2] = tot[t][3] = 0.f;
-  uint32_t u0[4], u1[4];
-  if (kb0 < kb1) {
-    dq4_load<NG>(w0 + (size_t)kb0 * 64, c, u0);
-    dq4_load<NG>(w1 + (size_t)kb0 * 64, c, u1);
+  // whole stages of 256 columns
+  const int nst = (nkb + 1) / 2, kb0 = 2 * (int)((long long)rank * nst / S);
+  int kb1 = 2 * (int)((long long)(rank + 1) * nst / S);
+  if (kb1 > nkb) kb1 = nkb;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], DQ4_WARPS);
+    }
+    fence_mbar_init();
   }
-  for (int kb = kb0; kb < kb1; ++kb) {
-    uint32_t v0[4], v1[4];
-    if (kb + 1 < kb1) {
-      dq4_load<NG>(w0 + (size_t)(kb + 1) * 64, c, v0);
-      dq4_load<NG>(w1 + (size_t)(kb + 1) * 64, c, v1);
-    }
-    float f0[NG], f1[NG];
-#pragma unroll
-    for (int x = 0; x < NG; ++x) {
-      f0[x] = 16.f * dq4_scale(p.scales, p.scale_bf16, s0 + kb * NG + x);
-      f1[x] = 16.f * dq4_scale(p.scales, p.scale_bf16, s1 + kb * NG + x);
-    }
-    float acc[NT][NG][4];
-    uint32_t b[NT][16];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const int m = m0 + t * 8 + g;
-#pragma unroll
-      for (int y = 0; y < 4; ++y) {
-        const uint4 v = m < p.M ? __ldg(reinterpret_cast<const uint4*>(p.a + (size_t)m * p.K + kb * 128 + dq4_col<NG>(y, c)))
-                                : make_uint4(0, 0, 0, 0);
-        b[t][4 * y + 0] = __byte_perm(v.x, v.z, 0x5410);
-        b[t][4 * y + 1] = __byte_perm(v.x, v.z, 0x7632);
-        b[t][4 * y + 2] = __byte_perm(v.y, v.w, 0x5410);
-        b[t][4 * y + 3] = __byte_perm(v.y, v.w, 0x7632);
-      }
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        acc[t][x][0] = acc[t][x][1] = acc[t][x][2] = acc[t][x][3] = 0.f;
-#pragma unroll
-        for (int y = 0; y < 8 / NG; ++y) {
-          const int k = x * (8 / NG) + y;
-          dq4_mma(acc[t][x], 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, b[t][2 * k], b[t][2 * k + 1]);
-        }
-      }
-    }
-#pragma unroll
-    for (int y = 0; y < 4; ++y) {
-      const int x = y * NG / 4;
-      const uint32_t a00 = dq4_code<0>(u0[y]), a10 = dq4_code<0>(u1[y]), a01 = dq4_code<1>(u0[y]),
-                     a11 = dq4_code<1>(u1[y]), a02 = dq4_code<2>(u0[y]), a12 = dq4_code<2>(u1[y]),
-                     a03 = dq4_code<3>(u0[y]), a13 = dq4_code<3>(u1[y]);
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        dq4_mma(acc[t][x], a00, a10, a01, a11, b[t][4 * y], b[t][4 * y + 1]);
-        dq4_mma(acc[t][x], a02, a12, a03, a13, b[t][4 * y + 2], b[t][4 * y + 3]);
-      }
-    }
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int x = 0; x < NG; ++x) {
-        tot[t][0] = fmaf(acc[t][x][0], f0[x], tot[t][0]);
-        tot[t][1] = fmaf(acc[t][x][1], f0[x], tot[t][1]);
-        tot[t][2] = fmaf(acc[t][x][2], f1[x], tot[t][2]);
-        tot[t][3] = fmaf(acc[t][x][3], f1[x], tot[t][3]);
-      }
-#pragma unroll
-    for (int y = 0; y < 4; ++y) u0[y] = v0[y], u1[y] = v1[y];
-  }
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) red[warp][g + (e >> 1) * 8][t * 8 + 2 * c + (e & 1)] = tot[t][e];
   __syncthreads();
-  for (int i = threadIdx.x; i < 16 * 8 * NT; i += DQ4_THREADS) {
-    const int n = i & 15, m = i >> 4;
-    if (m0 + m >= p.M) break;
-    float v = p.bias ? __bfloat162float(p.bias[n0 + n]) : 0.f;
+  float tot[RT][NT][4];
 #pragma unroll
-    for (int w = 0; w < DQ4_WARPS; ++w) v += red[w][n][m];
-    p.out[(size_t)(m0 + m) * p.N + n0 + n] = __float2bfloat16_rn(v);
-  }
-}
-
-// 32 codes (16 bytes) a thread -> bf16
-__global__ void __launch_bounds__(256) dq4_expand_kernel(const uint8_t* __restrict__ w, const void* __restrict__ scales,
-                                                         int scale_bf16, int group, size_t n32,
-                                                         __nv_bfloat16* __restrict__ out) {
-  const int per = group / 32;
-  for (size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x; i < n32; i += (size_t)gridDim.x * blockDim.x) {
-    const uint4 v = __ldg(reinterpret_cast<const uint4*>(w) + i);
-    const float s = dq4_scale(scales, scale_bf16, i / per), o = -8.f * s;
-    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t r[4];
+    for (int t = 0; t < NT; ++t) tot[r][t][0] = tot[r][t][1] = tot[r][t][2] = tot[r][t][3] = 0.f;
+  bool ok = true;
+  if (warp == DQ4_WARPS) {
+    // ---------------- producer ----------------
+    const int n = (kb1 - kb0 + 1) / 2;  // stages of two blocks; the last may hold one
+    if (lane == 0) {
+      prefetch_tmap(&tmW);
+      const uint8_t* rec = OWN ? nullptr : p.rec + ((size_t)blockIdx.z * nst + kb0 / 2) * C::RECORD;
+      auto weights = [&](int i) {  // columns past K come as zeros and are not multiplied
+        const int st = i % C::STAGES;
+        mbar_arrive_expect_tx(&full[st], C::WBYTES + (OWN ? 0 : C::RECORD));
+        tma_load_2d(ring + st * C::STAGE, &tmW, &full[st], (kb0 + 2 * i) * 64, n0);
+      };
+      auto record = [&](int i) {
+        const int st = i % C::STAGES;
+        if (!OWN) dq4_bulk(ring + st * C::STAGE + C::WBYTES, rec + (size_t)i * C::RECORD, C::RECORD, &full[st]);
+      };
+      const int head = n < C::STAGES ? n : C::STAGES;
+      for (int i = 0; i < head; ++i) weights(i);
+      if (!OWN) asm volatile("griddepcontrol.wait;" ::: "memory");  // the weights do not wait for A's records
+      for (int i = 0; i < head; ++i) record(i);
+      for (int i = head; i < n && ok; ++i) {
+        ok = mbar_wait(&empty[i % C::STAGES], (i / C::STAGES - 1) & 1, 0x321);
+        if (!ok) break;
+        weights(i);
+        record(i);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ---------------- 16 RT weight rows a warp ----------------
+    const int wrow = warp * 16 * RT;
+    size_t srow[RT][2];  // scale blocks (NG scales) of the lane's rows
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        r[k] = pack_bf16x2(fmaf((float)((x[j] >> (8 * k)) & 15u), s, o), fmaf((float)((x[j] >> (8 * k + 4)) & 15u), s, o));
-      reinterpret_cast<uint4*>(out)[i * 4 + j] = make_uint4(r[0], r[1], r[2], r[3]);
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int n = n0 + wrow + r * 16 + e * 8 + pg;
+        srow[r][e] = (size_t)(n < p.N ? n : p.N - 1) * nkb + kb0;
+      }
+    const int nb = kb1 - kb0;
+    float sc[2][RT][2][NG], sn[2][RT][2][NG];  // this stage's scales and the next one's
+    auto fetch = [&](int i, float (&s)[2][RT][2][NG]) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) dq4_scales<NG, BF>(p.scales, srow[r][e] + (i + b < nb ? i + b : nb - 1), s[b][r][e]);
+    };
+    fetch(0, sc);
+    if (OWN) {
+      const int n = (nb + 1) / 2;
+      for (int i = threadIdx.x; i < n * C::RECORD / 16; i += DQ4_WARPS * 32)  // rows past M stay zeros
+        reinterpret_cast<uint4*>(recs)[i] = make_uint4(0, 0, 0, 0);
+      named_bar(1, DQ4_WARPS * 32);
+#pragma unroll 1
+      for (int x = warp; x < n * p.M; x += DQ4_WARPS) {
+        const int j = x / n, r = x - j * n;
+        dq4_put<NG, NT>(p.a + (size_t)j * p.K, (kb0 + 2 * r) * 128, p.K, j, recs + r * C::RECORD);
+      }
+      named_bar(1, DQ4_WARPS * 32);
+    }
+    for (int i = 0; i < nb; i += 2) {
+      const int st = (i >> 1) % C::STAGES;
+      if (ok) ok = warp_wait(&full[st], ((i >> 1) / C::STAGES) & 1, 0x322);
+      if (!ok) break;
+      const uint8_t* rec = OWN ? recs + (i >> 1) * C::RECORD : ring + st * C::STAGE + C::WBYTES;
+      if (i + 2 < nb) fetch(i + 2, sn);
+      const uint8_t* ws = ring + st * C::STAGE;
+      float sum[RT][NT][4];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sum[r][t][0] = sum[r][t][1] = sum[r][t][2] = sum[r][t][3] = 0.f;
+      // The stage's two blocks side by side (independent sums); a block past K
+      // has zeros on A's side and takes the last block's scales.
+#pragma unroll
+      for (int x = 0; x < NG; ++x) {
+        float acc[2][RT][NT][4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            const float2 v = *reinterpret_cast<const float2*>(rec + b * dq4_block(NG, NT) + 2048 * NT +
+                                                              (x * 8 * NT + t * 8 + 2 * c) * 4);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) acc[b][r][t][0] = acc[b][r][t][2] = v.x, acc[b][r][t][1] = acc[b][r][t][3] = v.y;
+          }
+        uint32_t w[2][RT][2][4 / NG];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // 128-byte rows, 16-byte chunk j of row n at j ^ (n % 8)
+              const uint8_t* rp = ws + (wrow + r * 16 + e * 8 + pg) * 128;
+              uint32_t(&d)[4 / NG] = w[b][r][e];
+              if (NG == 1) {
+                const uint4 v = *reinterpret_cast<const uint4*>(rp + (((4 * b + c) ^ pg) << 4));
+                d[0] = v.x, d[1 % (4 / NG)] = v.y, d[2 % (4 / NG)] = v.z, d[3 % (4 / NG)] = v.w;
+              } else if (NG == 2) {
+                const uint2 v = *reinterpret_cast<const uint2*>(rp + (((4 * b + 2 * x + (c >> 1)) ^ pg) << 4) + (c & 1) * 8);
+                d[0] = v.x, d[1 % (4 / NG)] = v.y;
+              } else {
+                d[0] = *reinterpret_cast<const uint32_t*>(rp + (((4 * b + x) ^ pg) << 4) + 4 * c);
+              }
+            }
+#pragma unroll
+        for (int yy = 0; yy < 4 / NG; ++yy)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int y = x * (4 / NG) + yy;
+            uint32_t lo[RT][4], hi[RT][4];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+              const uint32_t a0 = w[b][r][0][yy], a1 = w[b][r][1][yy], a2 = a0 >> 8, a3 = a1 >> 8;
+              lo[r][0] = dq4_lo(a0), lo[r][1] = dq4_lo(a1), lo[r][2] = dq4_lo(a2), lo[r][3] = dq4_lo(a3);
+              hi[r][0] = dq4_hi(a0), hi[r][1] = dq4_hi(a1), hi[r][2] = dq4_hi(a2), hi[r][3] = dq4_hi(a3);
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+              const uint4 q = *reinterpret_cast<const uint4*>(rec + b * dq4_block(NG, NT) + ((t * 4 + y) * 32 + lane) * 16);
+#pragma unroll
+              for (int r = 0; r < RT; ++r) {
+                dq4_mma(acc[b][r][t], lo[r][0], lo[r][1], hi[r][0], hi[r][1], q.x, q.y);
+                dq4_mma(acc[b][r][t], lo[r][2], lo[r][3], hi[r][2], hi[r][3], q.z, q.w);
+              }
+            }
+          }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[r][t][e] = fmaf(acc[b][r][t][e], sc[b][r][e >> 1][x], sum[r][t][e]);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {  // out of the rows' powers of two
+        const float2 f = *reinterpret_cast<const float2*>(rec + 2 * dq4_block(NG, NT) + (t * 8 + 2 * c) * 4);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) tot[r][t][e] = fmaf(sum[r][t][e] * 1048576.f, e & 1 ? f.y : f.x, tot[r][t][e]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int x = 0; x < NG; ++x) sc[b][r][e][x] = sn[b][r][e][x];
     }
   }
+  // ---- partials [8 NT columns][ROWS] in the ring's place, added over the cluster in rank order ----
+  const bool failed = __syncthreads_or(!ok);
+  float* part = reinterpret_cast<float*>(ring);
+  if (failed) {  // (reported in the status word) copies under way land before the ring is given up
+    if (threadIdx.x == DQ4_WARPS * 32) {
+      const uint64_t t0 = globaltimer_ns();
+      for (int i = 0; i < C::STAGES; ++i)
+        for (int ph = 0; ph < 2; ++ph)
+          while (!mbar_try_wait(smem_u32(&full[i]), ph) && globaltimer_ns() - t0 < 10000000ull) {
+          }
+    }
+  } else if (warp < DQ4_WARPS) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          part[(t * 8 + 2 * c + (e & 1)) * (C::ROWS + 1) + warp * 16 * RT + r * 16 + (e >> 1) * 8 + pg] = tot[r][t][e];
+  }
+  if (S > 1)
+    cluster_sync();
+  else
+    __syncthreads();
+  const int lp = 31 - __clz(C::ROWS / S);  // this CTA's share: ROWS / S rows
+  const int cols = p.M - (int)blockIdx.z * 8 * NT < 8 * NT ? p.M - (int)blockIdx.z * 8 * NT : 8 * NT;
+  for (int i = threadIdx.x; i < cols << lp; i += DQ4_THREADS) {
+    const int j = i >> lp, n = (rank << lp) + (i - (j << lp)), m = blockIdx.z * 8 * NT + j;
+    if (failed || n0 + n >= p.N) continue;
+    const int at = j * (C::ROWS + 1) + n;
+    float v = part[at];
+    if (S > 1) {
+      const uint32_t a = smem_u32(part + at);
+      float x[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r) x[r] = r < S ? ld_cluster(a, r) : 0.f;  // all under way before the first is added
+      v = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+    }
+    if (p.bias) v += __bfloat162float(p.bias[n0 + n]);
+    p.out[(size_t)m * p.N + n0 + n] = __float2bfloat16_rn(v);
+  }
+  if (S > 1) cluster_sync();  // the others have read this CTA's partials
 }
 
-template <int NG>
-static void dq4_stream(const Dq4Args& p, cudaStream_t st) {
-  if (p.M <= 8)
-    dq4_stream_kernel<NG, 1><<<dim3(p.N / 16, 1), DQ4_THREADS, 0, st>>>(p);
-  else if (p.M <= 16)
-    dq4_stream_kernel<NG, 2><<<dim3(p.N / 16, 1), DQ4_THREADS, 0, st>>>(p);
-  else
-    dq4_stream_kernel<NG, 4><<<dim3(p.N / 16, (p.M + 31) / 32), DQ4_THREADS, 0, st>>>(p);
+// Eight codes (4 bytes) -> 16 bytes of bf16 per thread and step, four steps
+// under way: a warp reads and writes whole lines. Bound by 2.5 bytes a weight.
+__global__ void __launch_bounds__(256) dq4_expand_kernel(const uint32_t* __restrict__ w, const void* __restrict__ scales,
+                                                         int scale_bf16, int shift, size_t n8, uint4* __restrict__ out) {
+  const size_t stride = (size_t)gridDim.x * blockDim.x;
+  auto put = [&](size_t i, uint32_t v, float s) {
+    uint32_t r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // 2^23 + code and back: exact; (code - 8) * scale is rounded once more to bf16
+      const float a = (__uint_as_float(((v >> (8 * k)) & 15u) | 0x4B000000u) - 8388616.f) * s;
+      const float b = (__uint_as_float(((v >> (8 * k + 4)) & 15u) | 0x4B000000u) - 8388616.f) * s;
+      r[k] = pack_bf16x2(a, b);
+    }
+    out[i] = make_uint4(r[0], r[1], r[2], r[3]);
+  };
+  size_t i = blockIdx.x * (size_t)blockDim.x + threadIdx.x;
+  for (; i + 3 * stride < n8; i += 4 * stride) {
+    uint32_t v[4];
+    float s[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      v[u] = __ldg(w + i + u * stride);
+      s[u] = dq4_scale(scales, scale_bf16, (i + u * stride) >> shift);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) put(i + u * stride, v[u], s[u]);
+  }
+  for (; i < n8; i += stride) put(i, __ldg(w + i), dq4_scale(scales, scale_bf16, i >> shift));
+}
+
+// row tiles of 8 that a launch takes at once
+static int dq4_nt(int M) { return M <= 8 ? 1 : M <= 16 ? 2 : 4; }
+// CTAs of a cluster (see above) for `tiles` x `chunks` of 128 rows x 8 NT
+static int dq4_splits(int tiles, int chunks, int K) {
+  int S = 1;
+  while (S < 8 && (int64_t)tiles * chunks * S * 2 <= 2 * sm_count() && K / 256 >= 2 * S) S *= 2;
+  return S;
+}
+static bool dq4_own(int M, int K, int S) {
+  const int cols = ((K + 255) / 256 + S - 1) / S * 256;
+  return M <= 8 && cols <= DQ4_OWN_RECORDS * 256 && M * cols <= DQ4_OWN;
+}
+static uint64_t dq4_records_bytes(int M, int K) {  // for groups of 32, the largest
+  const int nt = dq4_nt(M), chunks = (M + 8 * nt - 1) / (8 * nt);
+  return (uint64_t)chunks * ((K + 255) / 256) * dq4_record(4, nt);
+}
+
+template <int NG, int NT, bool BF, bool OWN>
+static int dq4_launch(const void* Wq, Dq4Args p, uint8_t* ws, cudaStream_t st) {
+  using C = Dq4Cfg<NG, NT, OWN>;
+  static std::atomic<bool> attr[kMaxDevices];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= kMaxDevices) return set_error(LTXB_EINVAL, "dq4_gemm: device %d out of range", dev);
+  if (!attr[dev].load(std::memory_order_acquire)) {
+    cudaError_t e = cudaFuncSetAttribute(dq4_stream_kernel<NG, NT, BF, OWN>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return set_cuda_error(e, "dq4_gemm: cudaFuncSetAttribute");
+    attr[dev].store(true, std::memory_order_release);
+  }
+  const int chunks = (p.M + 8 * NT - 1) / (8 * NT), tiles = (p.N + C::ROWS - 1) / C::ROWS;
+  CUtensorMap tm;
+  if (int rc = make_tmap_2d(&tm, Wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K / 2, p.N, p.K / 2, 128, C::ROWS, CU_TENSOR_MAP_SWIZZLE_128B))
+    return rc;
+  cudaError_t e;
+  if (!OWN) {
+    p.rec = ws;
+    const int tasks = chunks * 8 * NT * ((p.K + 255) / 256);
+    dq4_rows_kernel<NG, NT><<<(tasks + 7) / 8, 256, 0, st>>>(p.a, p.M, p.K, tasks, ws);
+    launched();
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return set_cuda_error(e, "dq4_gemm rows");
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(tiles, p.splits, chunks);
+  cfg.blockDim = dim3(DQ4_THREADS);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute la[2];
+  la[0].id = cudaLaunchAttributeClusterDimension;
+  la[0].val.clusterDim.x = 1;
+  la[0].val.clusterDim.y = p.splits;
+  la[0].val.clusterDim.z = 1;
+  la[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  la[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = la;
+  cfg.numAttrs = OWN ? 1 : 2;
+  e = cudaLaunchKernelEx(&cfg, dq4_stream_kernel<NG, NT, BF, OWN>, tm, p);
+  launched();
+  return e == cudaSuccess ? LTXB_OK : set_cuda_error(e, "dq4_gemm launch");
+}
+
+template <int NG, bool BF>
+static int dq4_stream(const void* Wq, Dq4Args p, void* workspace, cudaStream_t st) {
+  const int nt = dq4_nt(p.M);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.splits = dq4_splits((p.N + 127) / 128, (p.M + 8 * nt - 1) / (8 * nt), p.K);
+  if (nt == 1)
+    return dq4_own(p.M, p.K, p.splits) ? dq4_launch<NG, 1, BF, true>(Wq, p, ws, st) : dq4_launch<NG, 1, BF, false>(Wq, p, ws, st);
+  if (nt == 2) return dq4_launch<NG, 2, BF, false>(Wq, p, ws, st);
+  return dq4_launch<NG, 4, BF, false>(Wq, p, ws, st);
 }
 
 }  // namespace ltxb
@@ -208,7 +539,10 @@ using namespace ltxb;
 extern "C" {
 
 uint64_t ltxb_dq4_gemm_workspace_bytes(int M, int N, int K) {
-  return M > DQ4_STREAM_ROWS && N > 0 && K > 0 ? (uint64_t)N * K * 2 : 0;
+  if (M <= 0 || N <= 0 || K < 128) return 0;
+  if (M > DQ4_STREAM_ROWS) return (uint64_t)N * K * 2;
+  const int nt = dq4_nt(M);
+  return dq4_own(M, K, dq4_splits((N + 127) / 128, (M + 8 * nt - 1) / (8 * nt), K)) ? 0 : dq4_records_bytes(M, K);
 }
 
 int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_dtype, int group, const void* bias,
@@ -225,11 +559,12 @@ int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_d
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int sb = scale_dtype == LTXB_DT_BF16;
   cudaError_t e;
+  const uint64_t need = ltxb_dq4_gemm_workspace_bytes(M, N, K);
+  if (need && (!workspace || workspace_bytes < need))
+    return set_error(LTXB_EINVAL, "dq4_gemm: workspace of %llu bytes is smaller than the %llu required",
+                     (unsigned long long)workspace_bytes, (unsigned long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 15) return set_error(LTXB_EINVAL, "dq4_gemm: workspace must be 16-byte aligned");
   if (M > DQ4_STREAM_ROWS) {
-    const uint64_t need = ltxb_dq4_gemm_workspace_bytes(M, N, K);
-    if (!workspace || workspace_bytes < need)
-      return set_error(LTXB_EINVAL, "dq4_gemm: workspace of %llu bytes is smaller than the %llu required",
-                       (unsigned long long)workspace_bytes, (unsigned long long)need);
     GemmArgs g{};
     g.A = A;
     g.lda = K;
@@ -243,27 +578,26 @@ int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_d
     g.out = out;
     g.ldo = N;
     if (int rc = gemm_check(g, nullptr)) return rc;  // before the expansion is launched
-    const size_t n32 = (size_t)N * K / 32;
-    int grid = (int)((n32 + 255) / 256);
-    if (grid > 8 * sm_count()) grid = 8 * sm_count();
-    dq4_expand_kernel<<<grid, 256, 0, st>>>(static_cast<const uint8_t*>(Wq), scales, sb, group, n32,
-                                            static_cast<__nv_bfloat16*>(workspace));
+    const size_t n8 = (size_t)N * K / 8;
+    const size_t ctas = (n8 + 255) / 256, most = 8 * (size_t)sm_count();
+    dq4_expand_kernel<<<(unsigned)(ctas < most ? ctas : most), 256, 0, st>>>(
+        static_cast<const uint32_t*>(Wq), scales, sb, group == 128 ? 4 : group == 64 ? 3 : 2, n8, static_cast<uint4*>(workspace));
     launched();
     e = cudaGetLastError();
     if (e != cudaSuccess) return set_cuda_error(e, "dq4_gemm expansion");
     return gemm_tc(g, st);
   }
-  Dq4Args p{static_cast<const __nv_bfloat16*>(A), static_cast<const uint8_t*>(Wq), scales,
-            static_cast<const __nv_bfloat16*>(bias), static_cast<__nv_bfloat16*>(out), M, N, K, sb};
-  if (group == 128)
-    dq4_stream<1>(p, st);
-  else if (group == 64)
-    dq4_stream<2>(p, st);
-  else
-    dq4_stream<4>(p, st);
-  launched();
-  e = cudaGetLastError();
-  return e == cudaSuccess ? LTXB_OK : set_cuda_error(e, "dq4_gemm");
+  Dq4Args p{};
+  p.scales = scales;
+  p.bias = static_cast<const __nv_bfloat16*>(bias);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.a = static_cast<const __nv_bfloat16*>(A);
+  if (group == 128) return sb ? dq4_stream<1, true>(Wq, p, workspace, st) : dq4_stream<1, false>(Wq, p, workspace, st);
+  if (group == 64) return sb ? dq4_stream<2, true>(Wq, p, workspace, st) : dq4_stream<2, false>(Wq, p, workspace, st);
+  return sb ? dq4_stream<4, true>(Wq, p, workspace, st) : dq4_stream<4, false>(Wq, p, workspace, st);
 }
 
 }  // extern "C"

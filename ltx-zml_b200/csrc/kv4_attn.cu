@@ -194,7 +194,8 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
   constexpr int MT = R == 8 ? 4 : 2;        // tiles of 16 tokens whose scores are held at once
   constexpr int PAIRS = KV4_PAGE * 4 * NG;  // bytes of a page's K or V pairs
   extern __shared__ __align__(128) uint8_t ka_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ka_raw) + 127) & ~uintptr_t(127));
+  // (aligned by an offset: through an integer the pointer would lose its address space)
+  uint8_t* ring = ka_raw + (-smem_u32(ka_raw) & 127u);
   KaSmem<R>& sm = *reinterpret_cast<KaSmem<R>*>(ring + NW * BLK);
   const int tid = threadIdx.x, warp = warp_id(), lane = lane_id(), g = lane >> 2, cq = lane & 3;
   const int Hq = a.c.heads * a.G;

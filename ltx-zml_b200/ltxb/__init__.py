@@ -1043,27 +1043,31 @@ def dq4_gemm(a, wq, scales, bias=None, out=None, workspace=None, stream=None) ->
     """a [M, K] bf16 . dequant(wq uint8 [N, K / 2], scales [N, K / group] f32 or
     bf16)^T (+ bias bf16) -> bf16 [M, N]: the linear with 4-bit weights
     (quantize_g4), the group being K over the scales' columns."""
-    M, K = a.shape
-    N = wq.shape[0]
     dev = a.device
-    if (a.dtype != torch.bfloat16 or wq.dtype != torch.uint8 or tuple(wq.shape) != (N, K // 2)
-            or scales.dtype not in (torch.bfloat16, torch.float32) or scales.shape[0] != N or K % scales.shape[1]):
+    if a.dim() != 2 or wq.dim() != 2 or scales.dim() != 2 or a.dtype != torch.bfloat16 or wq.dtype != torch.uint8:
         raise LtxbError(EINVAL, "dq4_gemm: a bf16 [M, K], wq uint8 [N, K / 2], scales f32 or bf16 [N, K / group]")
-    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,)):
-        raise LtxbError(EINVAL, f"dq4_gemm: bias must be bf16 [{N}]")
+    M, K = a.shape
+    N, half = wq.shape
+    rows, groups = scales.shape
+    bf = scales.dtype == torch.bfloat16
+    if half * 2 != K or rows != N or groups < 1 or K % groups or not (bf or scales.dtype == torch.float32):
+        raise LtxbError(EINVAL, "dq4_gemm: a bf16 [M, K], wq uint8 [N, K / 2], scales f32 or bf16 [N, K / group]")
+    if bias is not None and (bias.dtype != torch.bfloat16 or tuple(bias.shape) != (N,) or bias.device != dev):
+        raise LtxbError(EINVAL, f"dq4_gemm: bias must be bf16 [{N}] on {dev}")
+    if wq.device != dev or scales.device != dev:
+        raise LtxbError(EINVAL, "dq4_gemm: tensors on different devices")
     if out is None:
         out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
-    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N):
-        raise LtxbError(EINVAL, f"dq4_gemm: out must be bf16 [{M}, {N}]")
-    for t in (wq, scales, bias, out, workspace):
-        if t is not None and t.device != dev:
-            raise LtxbError(EINVAL, "dq4_gemm: tensors on different devices")
-    if workspace is None:
-        workspace = _scratch(lib.ltxb_dq4_gemm_workspace_bytes(M, N, K), dev, stream)
+    elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N) or out.device != dev:
+        raise LtxbError(EINVAL, f"dq4_gemm: out must be bf16 [{M}, {N}] on {dev}")
     with _device(dev):
-        _check(lib.ltxb_dq4_gemm(_ptr(a), _ptr(wq), _ptr(scales), DT_BF16 if scales.dtype == torch.bfloat16 else DT_F32,
-                                 K // scales.shape[1], _ptr(bias), _ptr(out), M, N, K, _ptr(workspace),
-                                 0 if workspace is None else workspace.numel(), _stream_on(stream, dev)))
+        if workspace is None:  # its size goes by the device's number of SMs
+            workspace = _scratch(lib.ltxb_dq4_gemm_workspace_bytes(M, N, K), dev, stream)
+        elif workspace.device != dev:
+            raise LtxbError(EINVAL, "dq4_gemm: tensors on different devices")
+        _check(lib.ltxb_dq4_gemm(_ptr(a), _ptr(wq), _ptr(scales), DT_BF16 if bf else DT_F32, K // groups, _ptr(bias),
+                                 _ptr(out), M, N, K, _ptr(workspace), 0 if workspace is None else workspace.numel(),
+                                 _stream_on(stream, dev)))
     return out
 
 
