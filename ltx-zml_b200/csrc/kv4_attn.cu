@@ -132,7 +132,7 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 struct KaSeg {
   int b, rt, h, pa, pb;
   int pages, tiles, len, first, count;  // of sequence b
-  long long left;                       // pages of the CTA's piece from pa on
+  int left;                             // pages of the CTA's piece from pa on
 };
 
 template <int R>
@@ -143,7 +143,7 @@ __device__ __forceinline__ void ka_seq(const KaArgs& a, KaSeg& k) {
   k.tiles = k.pages > 0 ? (k.count * a.G + R - 1) / R : 0;
 }
 __device__ __forceinline__ void ka_end(KaSeg& k) {
-  k.pb = k.pages - k.pa < k.left ? k.pages : k.pa + (int)k.left;
+  k.pb = k.pages - k.pa < k.left ? k.pages : k.pa + k.left;
 }
 // The next item of the CTA's piece; false behind its last.
 template <int R>
@@ -177,7 +177,7 @@ struct KaSmem {
   KaSeg at;
   KaSeg ls[KA_WARPS];
   int lp[KA_WARPS];
-  long long scan[KA_WARPS];
+  int scan[KA_WARPS], items[KA_WARPS];
   int found[4];
 };
 template <int R>
@@ -208,25 +208,38 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
     fence_mbar_init();
     sm.found[0] = -1;
   }
-  // ---- this CTA's piece of the line of pages ----
-  auto units = [&](int b) -> long long {
+  // ---- this CTA's piece of the line of pages (the host has made sure that it is shorter than 2^31) ----
+  auto units = [&](int b, int* items) -> int {
     KaSeg k;
     k.b = b;
     ka_seq<R>(a, k);
-    return (long long)k.pages * k.tiles * a.c.heads;
+    *items = k.tiles * a.c.heads;
+    return k.pages * *items;
   };
-  long long mine = 0;
-  for (int b = tid; b < a.c.batch; b += THREADS) mine += units(b);
+  int mine = 0, items = 0, n0 = 0;  // n0: pages of the thread's first sequence
+  for (int b = tid; b < a.c.batch; b += THREADS) {
+    int it;
+    const int n = units(b, &it);
+    if (b == tid) n0 = n;
+    mine += n;
+    items += it;
+  }
+  int upto = mine;  // inclusive over the warp's lanes
 #pragma unroll
-  for (int s = 16; s; s >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, s);
-  if (lane == 0) sm.scan[warp] = mine;
+  for (int s = 1; s < 32; s <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, upto, s);
+    if (lane >= s) upto += y;
+    items += __shfl_xor_sync(0xffffffffu, items, s);
+  }
+  if (lane == 31) sm.scan[warp] = upto;
+  if (lane == 0) sm.items[warp] = items;
   __syncthreads();
-  long long total = 0;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) total += sm.scan[w];
-  // at least a page for every warp of a CTA
-  const long long most = (total + NW - 1) / NW;
-  const int ctas = most < gridDim.x ? (int)most : (int)gridDim.x;
+  const int total = sm.scan[0] + sm.scan[1] + sm.scan[2] + sm.scan[3];
+  items = sm.items[0] + sm.items[1] + sm.items[2] + sm.items[3];
+  // a CTA for every item, or at least a page for every warp of a CTA, within the grid
+  int ctas = (total + NW - 1) / NW;
+  if (ctas < items) ctas = items;
+  if (ctas > (int)gridDim.x) ctas = gridDim.x;
   // sequences without tokens: their rows attend to nothing and are zero
   for (int b = blockIdx.x; b < a.c.batch; b += gridDim.x) {
     int first, count;
@@ -240,35 +253,44 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
     if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
     return;
   }
-  const long long u0 = total * blockIdx.x / ctas, u1 = total * (blockIdx.x + 1) / ctas;
-  {  // the sequence that holds u0: prefix sums over THREADS sequences at a time
-    long long base = 0;
-    for (int b0 = 0;; b0 += THREADS) {
-      const long long n = b0 + tid < a.c.batch ? units(b0 + tid) : 0;
-      long long x = n;
+  // pieces of `each` pages, the first `longer` of one page more
+  const int each = total / ctas, longer = total - each * ctas;
+  const int u0 = (int)blockIdx.x * each + ((int)blockIdx.x < longer ? (int)blockIdx.x : longer);
+  const int u1 = u0 + each + ((int)blockIdx.x < longer ? 1 : 0);
+  {  // the sequence that holds u0
+    auto found = [&](int b, int d) {
+      KaSeg k;
+      k.b = b;
+      ka_seq<R>(a, k);
+      const int item = d / k.pages;
+      sm.found[0] = b;
+      sm.found[1] = item / a.c.heads;
+      sm.found[2] = item % a.c.heads;
+      sm.found[3] = d - item * k.pages;
+    };
+    int base = 0;
+    if (a.c.batch <= THREADS) {  // a thread has one sequence, whose place the first scan gives
+      for (int w = 0; w < warp; ++w) base += sm.scan[w];
+      const int x = base + upto;
+      if (n0 > 0 && u0 >= x - n0 && u0 < x) found(tid, u0 - (x - n0));
+    } else {
+      for (int b0 = 0; base <= u0 && b0 < a.c.batch; b0 += THREADS) {
+        int it;
+        const int n = b0 + tid < a.c.batch ? units(b0 + tid, &it) : 0;
+        int x = n;
 #pragma unroll
-      for (int s = 1; s < 32; s <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, x, s);
-        if (lane >= s) x += y;
+        for (int s = 1; s < 32; s <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, s);
+          if (lane >= s) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) sm.scan[warp] = x;
+        __syncthreads();
+        for (int w = 0; w < warp; ++w) x += sm.scan[w];
+        x += base;
+        if (n > 0 && u0 >= x - n && u0 < x) found(b0 + tid, u0 - (x - n));
+        base += sm.scan[0] + sm.scan[1] + sm.scan[2] + sm.scan[3];
       }
-      __syncthreads();
-      if (lane == 31) sm.scan[warp] = x;
-      __syncthreads();
-      for (int w = 0; w < warp; ++w) x += sm.scan[w];
-      x += base;
-      if (n > 0 && u0 >= x - n && u0 < x) {
-        const long long d = u0 - (x - n);
-        KaSeg k;
-        k.b = b0 + tid;
-        ka_seq<R>(a, k);
-        sm.found[0] = k.b;
-        sm.found[1] = (int)(d / ((long long)k.pages * a.c.heads));
-        sm.found[2] = (int)(d / k.pages % a.c.heads);
-        sm.found[3] = (int)(d % k.pages);
-      }
-#pragma unroll
-      for (int w = 0; w < NW; ++w) base += sm.scan[w];
-      if (base > u0 || b0 >= a.c.batch) break;
     }
     __syncthreads();
     if (sm.found[0] < 0) {  // only if the lengths changed while this ran
@@ -687,11 +709,9 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
       int4 cut = make_int4(-1, 0, 0, 0);
       if (!next && was.pa == 0 && was.pb != was.pages) {
         // the item's last page on the line of pages, and the CTA that has it
-        const long long end = u1 - 1 + (was.pages - was.pb);
-        long long z = (end * ctas) / total;
-        while (total * (z + 1) / ctas <= end) ++z;
-        while (total * z / ctas > end) --z;
-        cut = make_int4(was.b, was.rt, was.h, (int)z);
+        const int end = u1 - 1 + (was.pages - was.pb), head = longer * (each + 1);
+        const int z = end < head ? end / (each + 1) : longer + (end - head) / each;
+        cut = make_int4(was.b, was.rt, was.h, z);
       }
       if (!next) a.cut[blockIdx.x] = cut;
     }
@@ -907,6 +927,9 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
     if (int rc = kv4_prepare(a.c, t, q, (size_t)ldq, cache->group, st)) return rc;
     return kv4_attention_tc(a.c, t, gate, out, a.causal, st);
   }
+  const int64_t tiles = (int64_t)rows * a.G / R + a.c.batch;  // at least the row tiles of all sequences
+  if ((int64_t)((a.c.cap + KV4_PAGE - 1) / KV4_PAGE) * a.c.heads > INT32_MAX / tiles)
+    return set_error(LTXB_EINVAL, "kv4 attention: more than 2^31 pages of work in a call (max_len bounds it)");
   a.cut = static_cast<int4*>(workspace);
   a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)ka_ctas(R, cache->group) * 16);
   const int ng = KV4_D / cache->group;
