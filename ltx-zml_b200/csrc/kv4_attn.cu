@@ -797,9 +797,10 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const KaArgs a) {
 // ---------------------------------------------------------------------------
 
 // Many rows a sequence and K/V head: the tcgen05 kernel over f16 operands in
-// the workspace. Below this the page kernel above, which reads the cache once
-// per 16 rows, is faster than laying the operands out.
-constexpr int KV4_TC_MIN = 64;
+// the workspace. Below this the page kernel above, whose time grows with every
+// 16 rows, is faster than laying the operands out (4 x 16,384 tokens x 8 heads:
+// 33 us per 16 rows against 165 for up to 256).
+constexpr int KV4_TC_MIN = 80;
 constexpr uint64_t KV4_TC_BYTES = 24ull << 30;  // and never for operands beyond this
 
 static uint64_t kv4_tc_layout(const Kv4View& c, int G, Kv4Tc* t, void* ws) {

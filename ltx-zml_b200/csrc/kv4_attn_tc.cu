@@ -500,15 +500,21 @@ static long long kt_tiles(const Kv4View& c, int G) {
 }
 
 int kv4_tc_splits(const Kv4View& c, int G) {
-  // time ~ waves x key tiles per split, a split adding one f32 state per row to write and read (about 3 %)
-  // the same with and without row_start: the workspace is sized before that is known
+  // In key tiles of 128 (1.65 us each here): waves of CTAs times their tiles and
+  // about three more for starting and ending, and with splits the f32 states
+  // (512 bytes per row, head and split, written and read at 6.5 TB/s, 1e-4 of a
+  // tile). 3,520 x 28,160 tokens, 32 heads: 4 splits 1.66 ms, none 1.95; four
+  // causal prompts of 1,500 tokens: none 0.13 ms, 8 splits 0.41. Tiles are
+  // counted alike with and without row_start: the workspace is sized before
+  // that is known.
   const long long tiles = (long long)c.rows * G / KV4_TC_ROWS + (c.batch < c.rows ? c.batch : c.rows);
   const long long units = tiles * c.heads;
   const int nkv = (c.cap + KT_N - 1) / KT_N, sms = sm_count();
   int best = 1;
   double best_t = 0;
   for (int s = 1; s <= 8 && s <= nkv; ++s) {
-    const double t = (double)((units * s + sms - 1) / sms) * ((nkv + s - 1) / s) * (1.0 + 0.03 * (s - 1));
+    const double waves = (double)((units * s + sms - 1) / sms);
+    const double t = waves * ((nkv + s - 1) / s + 3) + (s > 1 ? 1e-4 * s * c.rows * G * c.heads : 0.0);
     if (s == 1 || t < best_t) {
       best = s;
       best_t = t;
