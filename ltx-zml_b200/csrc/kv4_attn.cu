@@ -26,14 +26,15 @@
 // accumulators are f32.
 //
 // Work is split by pages, not by sequence: all (sequence, head, row tile)
-// items laid end to end are one line of pages, each CTA takes an equal piece
-// of it, its warps take the pages of an item in turn, and a second kernel
+// items laid end to end are one line of pages (each item with KA_ITEM more, what
+// starting and ending it costs: without them a batch of 64 sequences of 17 to
+// 8,192 tokens took 173 us instead of 103), each CTA takes an equal piece of it, its warps take the pages of an item in turn, and a second kernel
 // joins the items that were cut (in page order, so results do not depend on
 // timing). Lengths are read on the device only. A warp has room for one
 // (page, head) block of its own: the next page's K (codes and pairs, two bulk
 // copies) arrives while it works on V, the next V while it works on K, and no
-// barrier joins the warps until an item ends. 16 warps an SM (12 with groups
-// of 32, or 16 rows) keep about 70 KB per SM in flight.
+// barrier joins the warps until an item ends. (Two buffers each for K and V
+// gained nothing: the loads alone take 95 us of 131,009 tokens' 114.)
 //
 // A token whose V group is stored as NaN, or whose page number is bad, makes
 // every row that attends to it NaN and no others: where a page holds tokens
@@ -132,8 +133,9 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 struct KaSeg {
   int b, rt, h, pa, pb;
   int pages, tiles, len, first, count;  // of sequence b
-  int left;                             // pages of the CTA's piece from pa on
+  int left, lead;                       // places of the CTA's piece from here on, and those before page pa
 };
+constexpr int KA_ITEM = 10;  // places on the line that an item takes besides its pages
 
 template <int R>
 __device__ __forceinline__ void ka_seq(const KaArgs& a, KaSeg& k) {
@@ -142,14 +144,17 @@ __device__ __forceinline__ void ka_seq(const KaArgs& a, KaSeg& k) {
   k.pages = (k.len + KV4_PAGE - 1) / KV4_PAGE;
   k.tiles = k.pages > 0 ? (k.count * a.G + R - 1) / R : 0;
 }
+// pb from the places that are left; pb <= pa: none for a page
 __device__ __forceinline__ void ka_end(KaSeg& k) {
-  k.pb = k.pages - k.pa < k.left ? k.pages : k.pa + k.left;
+  const int n = k.left - k.lead;
+  k.pb = k.pages - k.pa < n ? k.pages : k.pa + n;
 }
 // The next item of the CTA's piece; false behind its last.
 template <int R>
 __device__ __forceinline__ bool ka_next(const KaArgs& a, KaSeg& k) {
-  k.left -= k.pb - k.pa;
-  if (k.left <= 0) return false;
+  k.left -= k.lead + k.pb - k.pa;
+  if (k.left <= KA_ITEM) return false;
+  k.lead = KA_ITEM;
   k.pa = 0;
   if (++k.h >= a.c.heads) {
     k.h = 0;
@@ -184,12 +189,12 @@ template <int R>
 constexpr int ka_smem_bytes(int ng) {
   return KA_WARPS * kv4_block(ng) + (int)sizeof(KaSmem<R>) + 128;
 }
-// CTAs an SM: four take 128 registers a thread and 52 KB each; 16 rows need
-// more registers, groups of 32 more of both.
-__host__ __device__ constexpr int ka_per_sm(int ng, int R) { return 3; }
+// CTAs an SM, of 168 registers a thread: with four and 128 registers 131,009
+// tokens x 32 heads took 125 us instead of 118
+constexpr int KA_PER_SM = 3;
 
 template <int NG, int R>
-__global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(const KaArgs a) {
+__global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const KaArgs a) {
   constexpr int NT = R / 8, BLK = kv4_block(NG), NW = KA_WARPS, THREADS = KA_THREADS;
   constexpr int MT = R == 8 ? 4 : 2;        // tiles of 16 tokens whose scores are held at once
   constexpr int PAIRS = KV4_PAGE * 4 * NG;  // bytes of a page's K or V pairs
@@ -214,7 +219,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
     k.b = b;
     ka_seq<R>(a, k);
     *items = k.tiles * a.c.heads;
-    return k.pages * *items;
+    return k.tiles > 0 ? (k.pages + KA_ITEM) * *items : 0;
   };
   int mine = 0, items = 0, n0 = 0;  // n0: pages of the thread's first sequence
   for (int b = tid; b < a.c.batch; b += THREADS) {
@@ -237,7 +242,7 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
   const int total = sm.scan[0] + sm.scan[1] + sm.scan[2] + sm.scan[3];
   items = sm.items[0] + sm.items[1] + sm.items[2] + sm.items[3];
   // a CTA for every item, or at least a page for every warp of a CTA, within the grid
-  int ctas = (total + NW - 1) / NW;
+  int ctas = (total - items * KA_ITEM + NW - 1) / NW;
   if (ctas < items) ctas = items;
   if (ctas > (int)gridDim.x) ctas = gridDim.x;
   // sequences without tokens: their rows attend to nothing and are zero
@@ -262,11 +267,11 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
       KaSeg k;
       k.b = b;
       ka_seq<R>(a, k);
-      const int item = d / k.pages;
+      const int item = d / (k.pages + KA_ITEM);
       sm.found[0] = b;
       sm.found[1] = item / a.c.heads;
       sm.found[2] = item % a.c.heads;
-      sm.found[3] = d - item * k.pages;
+      sm.found[3] = d - item * (k.pages + KA_ITEM);
     };
     int base = 0;
     if (a.c.batch <= THREADS) {  // a thread has one sequence, whose place the first scan gives
@@ -302,7 +307,9 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
       k.b = sm.found[0];
       k.rt = sm.found[1];
       k.h = sm.found[2];
-      k.pa = sm.found[3];
+      const int d = sm.found[3] - KA_ITEM;
+      k.pa = d > 0 ? d : 0;
+      k.lead = d > 0 ? 0 : -d;
       k.left = u1 - u0;
       ka_seq<R>(a, k);
       ka_end(k);
@@ -311,6 +318,10 @@ __global__ void __launch_bounds__(KA_THREADS, ka_per_sm(NG, R)) kv4_attn_kernel(
       if (tid == 0) sm.at = k;
     }
     __syncthreads();
+    if (sm.at.pb <= sm.at.pa) {  // a short piece, all of it before an item's first page
+      if (tid == 0) a.cut[blockIdx.x] = make_int4(-1, 0, 0, 0);
+      return;
+    }
   }
 
   // ---- loads (lane 0): this warp's pages in order; K of the next page, then its V ----
@@ -839,14 +850,21 @@ static bool kv4_use_tc(const Kv4View& c, int G, uint64_t* bytes, Kv4Tc* t) {
 // Query rows of a tile: 8 where every sequence's rows fit (one n8 tile of
 // the MMA), else 16, which unpacks a page once for twice the rows.
 static int ka_rows(int rows, int batch, int G) { return (int64_t)rows * G <= 8ll * batch ? 8 : 16; }
-static int ka_ctas(int R, int group) { return sm_count() * ka_per_sm(KV4_D / group, R); }
-static uint64_t ka_workspace(int R, int group) {
-  const uint64_t n = ka_ctas(R, group);
-  return n * 16 + n * 2 * R * (KV4_D + 2) * 4;
+// CTAs of a call: as many as the GPU holds at once, or as the capacity can keep
+// busy (one per item, a page per warp). Row tiles are bounded alike with and
+// without row_start: the workspace is sized before that is known.
+static int ka_ctas(const Kv4View& c, int G, int R) {
+  const int64_t items = ((int64_t)c.rows * G / R + (c.batch < c.rows ? c.batch : c.rows)) * c.heads;
+  const int64_t pages = (c.cap + KV4_PAGE - 1) / KV4_PAGE, most = (int64_t)sm_count() * KA_PER_SM;
+  if (items >= most || items * pages / KA_WARPS >= most) return (int)most;
+  const int64_t n = (items * pages + KA_WARPS - 1) / KA_WARPS;
+  return (int)(n > items ? n : items);
 }
+static uint64_t ka_cut_bytes(int ctas) { return ((uint64_t)ctas * 16 + 255) & ~uint64_t(255); }
+static uint64_t ka_workspace(int ctas, int R) { return ka_cut_bytes(ctas) + (uint64_t)ctas * 2 * R * (KV4_D + 2) * 4; }
 
 template <int NG, int R>
-static int ka_launch(const KaArgs& a, cudaStream_t st) {
+static int ka_launch(const KaArgs& a, int ctas, cudaStream_t st) {
   constexpr int bytes = ka_smem_bytes<R>(NG);
   static std::atomic<bool> attr[kMaxDevices];
   int dev = 0;
@@ -857,7 +875,6 @@ static int ka_launch(const KaArgs& a, cudaStream_t st) {
     if (e != cudaSuccess) return set_cuda_error(e, "kv4 attention: cudaFuncSetAttribute");
     attr[dev].store(true, std::memory_order_release);
   }
-  const int ctas = ka_ctas(R, KV4_D / NG);
   kv4_attn_kernel<NG, R><<<ctas, KA_THREADS, bytes, st>>>(a);
   launched();
   cudaError_t e = cudaGetLastError();
@@ -889,7 +906,8 @@ uint64_t ltxb_attention_kv4_workspace_bytes(const ltxb_kv4_cache* cache, int row
   c.rows = rows;
   uint64_t bytes;
   if (kv4_use_tc(c, H / c.heads, &bytes, &t)) return bytes;
-  return ka_workspace(ka_rows(rows, c.batch, H / c.heads), cache->group);
+  const int R = ka_rows(rows, c.batch, H / c.heads);
+  return ka_workspace(ka_ctas(c, H / c.heads, R), R);
 }
 
 int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, const void* q, int64_t ldq, void* out,
@@ -910,7 +928,8 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
   uint64_t need = 0;
   Kv4Tc t{};
   const bool tc = kv4_use_tc(a.c, a.G, &need, &t);
-  if (!tc) need = ka_workspace(R, cache->group);
+  const int ctas = ka_ctas(a.c, a.G, R);
+  if (!tc) need = ka_workspace(ctas, R);
   if (!workspace || workspace_bytes < need)
     return set_error(LTXB_EINVAL, "kv4 attention: workspace of %llu bytes is smaller than the %llu required",
                      (unsigned long long)workspace_bytes, (unsigned long long)need);
@@ -929,19 +948,19 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
     return kv4_attention_tc(a.c, t, gate, out, a.causal, st);
   }
   const int64_t tiles = (int64_t)rows * a.G / R + a.c.batch;  // at least the row tiles of all sequences
-  if ((int64_t)((a.c.cap + KV4_PAGE - 1) / KV4_PAGE) * a.c.heads > INT32_MAX / tiles)
+  if (((int64_t)(a.c.cap + KV4_PAGE - 1) / KV4_PAGE + KA_ITEM) * a.c.heads > INT32_MAX / tiles)
     return set_error(LTXB_EINVAL, "kv4 attention: more than 2^31 pages of work in a call (max_len bounds it)");
   a.cut = static_cast<int4*>(workspace);
-  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (size_t)ka_ctas(R, cache->group) * 16);
+  a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + ka_cut_bytes(ctas));
   const int ng = KV4_D / cache->group;
   if (R == 8) {
-    if (ng == 1) return ka_launch<1, 8>(a, st);
-    if (ng == 2) return ka_launch<2, 8>(a, st);
-    return ka_launch<4, 8>(a, st);
+    if (ng == 1) return ka_launch<1, 8>(a, ctas, st);
+    if (ng == 2) return ka_launch<2, 8>(a, ctas, st);
+    return ka_launch<4, 8>(a, ctas, st);
   }
-  if (ng == 1) return ka_launch<1, 16>(a, st);
-  if (ng == 2) return ka_launch<2, 16>(a, st);
-  return ka_launch<4, 16>(a, st);
+  if (ng == 1) return ka_launch<1, 16>(a, ctas, st);
+  if (ng == 2) return ka_launch<2, 16>(a, ctas, st);
+  return ka_launch<4, 16>(a, ctas, st);
 }
 
 }  // extern "C"

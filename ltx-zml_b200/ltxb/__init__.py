@@ -882,14 +882,14 @@ class _KV4(ctypes.Structure):
 
 def _row_tensor(t, heads: int, name: str, device) -> int:
     """Row stride of a [rows, heads, 128] bf16 CUDA tensor whose rows are contiguous."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1] != heads or t.shape[2] != 128:
+    if t.dtype is not torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (heads, 128):
         raise LtxbError(EINVAL, f"{name} must be bf16 [rows, {heads}, 128], got {t.dtype} {list(t.shape)}")
     if t.device != device:
         raise LtxbError(EINVAL, f"{name} is on {t.device}, the cache on {device}")
-    if t.stride(2) != 1 or (heads > 1 and t.stride(1) != 128):
+    row, head, one = t.stride()
+    if one != 1 or (head != 128 and heads > 1):
         raise LtxbError(EINVAL, f"{name}: a row's heads must be contiguous")
-    # one row has no stride of its own
-    return t.stride(0) if t.shape[0] > 1 else heads * 128
+    return row if t.shape[0] > 1 else heads * 128  # one row has no stride of its own
 
 
 def _index_tensor(t, shape, name: str, device) -> int | None:
@@ -942,10 +942,16 @@ class KV4Cache:
         self._c = _KV4(pages.data_ptr(), None if page_table is None else page_table.data_ptr(), seq_lens.data_ptr(),
                        pages.shape[0], self.kv_heads, group, self.batch, max_pages, int(max_len))
         self._ref = ctypes.byref(self._c)
+        self._need = {}  # workspace bytes of attention calls by (rows, H)
 
     def _call(self, fn, stream, *args) -> None:
-        with _device(self.device):
-            _check(fn(self._ref, *args, _stream_on(stream, self.device)))
+        if torch.cuda.current_device() == self.device.index:
+            rc = fn(self._ref, *args, _stream_on(stream, self.device))
+        else:  # the library runs on the current device
+            with torch.cuda.device(self.device):
+                rc = fn(self._ref, *args, _stream_on(stream, self.device))
+        if rc != OK:
+            _check(rc)
 
     def append(self, k, v, row_start=None, stream=None) -> None:
         """Quantise k, v [rows, kv_heads, 128] bf16 (rows may be strided) into the sequences' last tokens."""
@@ -962,14 +968,16 @@ class KV4Cache:
         if dtype not in (torch.bfloat16, torch.float32):
             raise LtxbError(EINVAL, "read: dtype must be bfloat16 or float32")
         if out is None:
-            both = torch.empty(2, rows, self.kv_heads, 128, dtype=dtype, device=self.device)
-            out = both[0], both[1]
-        for t in out:
-            if t.dtype != dtype or tuple(t.shape) != (rows, self.kv_heads, 128) or t.device != self.device:
-                raise LtxbError(EINVAL, f"read: outputs must be {dtype} [{rows}, {self.kv_heads}, 128] on {self.device}")
+            out = torch.empty(2, rows, self.kv_heads, 128, dtype=dtype, device=self.device).unbind(0)
+            kp, vp = out[0].data_ptr(), out[1].data_ptr()
+        else:
+            for t in out:
+                if t.dtype != dtype or tuple(t.shape) != (rows, self.kv_heads, 128) or t.device != self.device:
+                    raise LtxbError(EINVAL,
+                                    f"read: outputs must be {dtype} [{rows}, {self.kv_heads}, 128] on {self.device}")
+            kp, vp = _ptr(out[0]), _ptr(out[1])
         rs = _index_tensor(row_start, (self.batch + 1,), "row_start", self.device)
-        self._call(lib.ltxb_kv4_read, stream, rs, _ptr(out[0]), _ptr(out[1]),
-                   DT_F32 if dtype == torch.float32 else DT_BF16, rows)
+        self._call(lib.ltxb_kv4_read, stream, rs, kp, vp, DT_F32 if dtype is torch.float32 else DT_BF16, rows)
         return out
 
 
@@ -988,8 +996,10 @@ def attention_kv4(q, cache: KV4Cache, row_start=None, causal: bool = True, gate=
         raise LtxbError(EINVAL, f"gate must be f32 [{rows}, {H}] on {q.device}")
     rs = _index_tensor(row_start, (cache.batch + 1,), "row_start", cache.device)
     if workspace is None:
-        with _device(cache.device):  # its size goes by the device's number of SMs
-            need = lib.ltxb_attention_kv4_workspace_bytes(cache._ref, rows, H)
+        need = cache._need.get((rows, H))
+        if need is None:
+            with _device(cache.device):  # its size goes by the device's number of SMs
+                need = cache._need[rows, H] = lib.ltxb_attention_kv4_workspace_bytes(cache._ref, rows, H)
         workspace = _scratch(need, cache.device, stream)
     ws, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel())
     cache._call(lib.ltxb_attention_kv4, stream, rs, q.data_ptr(), ldq, _ptr(out), _ptr(gate), rows, H, int(causal),
