@@ -14,16 +14,23 @@
 //   sum_k x (c - 8) s = s (sum x c - 8 sum x)
 // needs one f32 FMA per group and output. Products are exact, sums f32.
 //
-// A CTA takes 128 weight rows and 1 / S of K: a producer warp streams
-// [128 rows x 128 bytes] tiles (TMA, 256 columns) through a ring, four warps
-// take 32 rows each (two M tiles, so that a B fragment is read once for both).
-// A's records (its values in the order of the B fragments, the groups' sums)
-// come through the same ring from a kernel of their own, which runs under this
-// one's start; where a CTA has few values of A (DQ4_OWN), its warps make them
-// in shared memory while the ring fills. The S CTAs of a cluster add their f32
-// partials in rank order through distributed shared memory. S fills the SMs
-// where N alone does not: the largest power of two up to 8 that keeps the CTAs
-// within what the SMs hold at once.
+// A CTA takes 128 weight rows (256 for 17 rows of A and more) and 1 / S of K: a
+// producer warp streams [rows x 128 bytes] tiles (TMA, 256 columns) through a
+// ring, eight warps take 16 (32) rows each, both 128-column blocks of a tile
+// side by side. A's records (its values in the order of the B fragments, the
+// groups' sums) come through the same ring from a kernel of their own, which
+// runs under this one's start; where a CTA has few values of A (DQ4_OWN), its
+// warps make them in shared memory while the ring fills. The S CTAs of a
+// cluster add their f32 partials in rank order through distributed shared
+// memory. S fills the SMs where N alone does not: the largest power of two up
+// to 8 that keeps the CTAs within what the SMs hold at once.
+// Measured: 2 x 36,864 x 4,096, groups of 64, f32 scales: 25 us (85 MB, 3.4
+// TB/s); 8 x 36,864 x 4,096, groups of 128: 24 us; 16 x 4,096 x 16,384, groups
+// of 32: 28 us; 16 x 16,384 x 4,096: 22 us. What bounds it there is the start
+// (A's records, first tiles: 3.5 us), the instructions of a tile (the scale
+// and start value of every group and output) and the cluster's sum (3 us), no
+// longer the bytes. (Four warps of
+// 32 rows each: 27, 27, 42 and 21 us.)
 //
 // More rows: the weights are expanded to bf16 in the workspace (one rounding:
 // the code and a bf16 scale have up to 11 significant bits) and multiplied by
@@ -170,11 +177,11 @@ __device__ __forceinline__ void dq4_bulk(void* dst, const void* src, uint32_t by
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
-  float v;
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
+  float4 v;
   asm volatile(
-      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.f32 %0, [a];\n\t}"
-      : "=f"(v)
+      "{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %4, %5;\n\tld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [a];\n\t}"
+      : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
       : "r"(addr), "r"(rank)
       : "memory");
   return v;
@@ -182,12 +189,12 @@ __device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
 
 template <int NG, int NT, bool OWN>
 struct Dq4Cfg {
-  static constexpr int ROWS = 128, RT = 1;
+  static constexpr int RT = NT == 4 ? 2 : 1, ROWS = 16 * RT * DQ4_WARPS;
   static constexpr int WBYTES = ROWS * 128, RECORD = dq4_record(NG, NT);
   static constexpr int STAGE = WBYTES + (OWN ? 0 : (RECORD + 1023) / 1024 * 1024);  // 1 KB: the swizzled tile's alignment
-  static constexpr int PER_SM = 2;
+  static constexpr int PER_SM = NT == 4 ? 1 : 2;  // CTAs an SM
   static constexpr int STAGES = 4;
-  static constexpr int PART = 8 * NT * (ROWS + 1) * 4;
+  static constexpr int PART = 8 * NT * (ROWS + 4) * 4;
   static constexpr int SMEM = STAGES * STAGE + (OWN ? DQ4_OWN_RECORDS * RECORD : 0) + 1024 + 256;
   static_assert(PART <= STAGES * STAGE, "the partials take the ring's place");
 };
@@ -403,28 +410,33 @@ __global__ void __launch_bounds__(DQ4_THREADS, Dq4Cfg<NG, NT, OWN>::PER_SM)
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          part[(t * 8 + 2 * c + (e & 1)) * (C::ROWS + 1) + warp * 16 * RT + r * 16 + (e >> 1) * 8 + pg] = tot[r][t][e];
+          part[(t * 8 + 2 * c + (e & 1)) * (C::ROWS + 4) + warp * 16 * RT + r * 16 + (e >> 1) * 8 + pg] = tot[r][t][e];
   }
   if (S > 1)
     cluster_sync();
   else
     __syncthreads();
-  const int lp = 31 - __clz(C::ROWS / S);  // this CTA's share: ROWS / S rows
+  const int lp = 29 - __clz(C::ROWS / S);  // this CTA's share: ROWS / S rows, four a thread
   const int cols = p.M - (int)blockIdx.z * 8 * NT < 8 * NT ? p.M - (int)blockIdx.z * 8 * NT : 8 * NT;
   for (int i = threadIdx.x; i < cols << lp; i += DQ4_THREADS) {
-    const int j = i >> lp, n = (rank << lp) + (i - (j << lp)), m = blockIdx.z * 8 * NT + j;
+    const int j = i >> lp, n = ((rank << lp) + (i - (j << lp))) * 4, m = blockIdx.z * 8 * NT + j;
     if (failed || n0 + n >= p.N) continue;
-    const int at = j * (C::ROWS + 1) + n;
-    float v = part[at];
+    const float* at = part + j * (C::ROWS + 4) + n;
+    float4 v = *reinterpret_cast<const float4*>(at);
     if (S > 1) {
-      const uint32_t a = smem_u32(part + at);
-      float x[8];
+      const uint32_t a = smem_u32(at);
+      float4 x[8];
 #pragma unroll
-      for (int r = 0; r < 8; ++r) x[r] = r < S ? ld_cluster(a, r) : 0.f;  // all under way before the first is added
-      v = ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
+      for (int r = 0; r < 8; ++r) x[r] = r < S ? ld_cluster4(a, r) : make_float4(0.f, 0.f, 0.f, 0.f);  // all under way at once
+      v = x[0];
+#pragma unroll
+      for (int r = 1; r < 8; ++r) v.x += x[r].x, v.y += x[r].y, v.z += x[r].z, v.w += x[r].w;
     }
-    if (p.bias) v += __bfloat162float(p.bias[n0 + n]);
-    p.out[(size_t)m * p.N + n0 + n] = __float2bfloat16_rn(v);
+    if (p.bias) {
+      const uint2 bb = __ldg(reinterpret_cast<const uint2*>(p.bias + n0 + n));
+      v.x += bf16_lo(bb.x), v.y += bf16_hi(bb.x), v.z += bf16_lo(bb.y), v.w += bf16_hi(bb.y);
+    }
+    *reinterpret_cast<uint2*>(p.out + (size_t)m * p.N + n0 + n) = make_uint2(pack_bf16x2(v.x, v.y), pack_bf16x2(v.z, v.w));
   }
   if (S > 1) cluster_sync();  // the others have read this CTA's partials
 }
@@ -462,10 +474,13 @@ __global__ void __launch_bounds__(256) dq4_expand_kernel(const uint32_t* __restr
 
 // row tiles of 8 that a launch takes at once
 static int dq4_nt(int M) { return M <= 8 ? 1 : M <= 16 ? 2 : 4; }
-// CTAs of a cluster (see above) for `tiles` x `chunks` of 128 rows x 8 NT
-static int dq4_splits(int tiles, int chunks, int K) {
+// CTAs of a cluster (see above)
+// weight rows of a CTA, and the CTAs an SM holds
+static int dq4_tile(int nt) { return nt == 4 ? 256 : 128; }
+static int dq4_splits(int N, int M, int K) {
+  const int nt = dq4_nt(M), tiles = (N + dq4_tile(nt) - 1) / dq4_tile(nt), chunks = (M + 8 * nt - 1) / (8 * nt);
   int S = 1;
-  while (S < 8 && (int64_t)tiles * chunks * S * 2 <= 2 * sm_count() && K / 256 >= 2 * S) S *= 2;
+  while (S < 8 && (int64_t)tiles * chunks * S * 2 <= (nt == 4 ? 1 : 2) * sm_count() && K / 256 >= 2 * S) S *= 2;
   return S;
 }
 static bool dq4_own(int M, int K, int S) {
@@ -494,9 +509,9 @@ static int dq4_launch(const void* Wq, Dq4Args p, uint8_t* ws, cudaStream_t st) {
   if (int rc = make_tmap_2d(&tm, Wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K / 2, p.N, p.K / 2, 128, C::ROWS, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   cudaError_t e;
+  const int tasks = chunks * 8 * NT * ((p.K + 255) / 256);
   if (!OWN) {
     p.rec = ws;
-    const int tasks = chunks * 8 * NT * ((p.K + 255) / 256);
     dq4_rows_kernel<NG, NT><<<(tasks + 7) / 8, 256, 0, st>>>(p.a, p.M, p.K, tasks, ws);
     launched();
     e = cudaGetLastError();
@@ -515,7 +530,9 @@ static int dq4_launch(const void* Wq, Dq4Args p, uint8_t* ws, cudaStream_t st) {
   la[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   la[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = la;
-  cfg.numAttrs = OWN ? 1 : 2;
+  // The early start pays while A's kernel is small: 8 x 36,864 x 4,096 24.0 us
+  // with it, 25.5 without; 16 x 4,096 x 16,384 (1,024 warps of A's) 33.0 and 27.7.
+  cfg.numAttrs = !OWN && tasks <= 512 ? 2 : 1;
   e = cudaLaunchKernelEx(&cfg, dq4_stream_kernel<NG, NT, BF, OWN>, tm, p);
   launched();
   return e == cudaSuccess ? LTXB_OK : set_cuda_error(e, "dq4_gemm launch");
@@ -525,7 +542,7 @@ template <int NG, bool BF>
 static int dq4_stream(const void* Wq, Dq4Args p, void* workspace, cudaStream_t st) {
   const int nt = dq4_nt(p.M);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.splits = dq4_splits((p.N + 127) / 128, (p.M + 8 * nt - 1) / (8 * nt), p.K);
+  p.splits = dq4_splits(p.N, p.M, p.K);
   if (nt == 1)
     return dq4_own(p.M, p.K, p.splits) ? dq4_launch<NG, 1, BF, true>(Wq, p, ws, st) : dq4_launch<NG, 1, BF, false>(Wq, p, ws, st);
   if (nt == 2) return dq4_launch<NG, 2, BF, false>(Wq, p, ws, st);
@@ -541,8 +558,7 @@ extern "C" {
 uint64_t ltxb_dq4_gemm_workspace_bytes(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K < 128) return 0;
   if (M > DQ4_STREAM_ROWS) return (uint64_t)N * K * 2;
-  const int nt = dq4_nt(M);
-  return dq4_own(M, K, dq4_splits((N + 127) / 128, (M + 8 * nt - 1) / (8 * nt), K)) ? 0 : dq4_records_bytes(M, K);
+  return dq4_own(M, K, dq4_splits(N, M, K)) ? 0 : dq4_records_bytes(M, K);
 }
 
 int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_dtype, int group, const void* bias,

@@ -456,10 +456,10 @@ done:
 // One warp per (row, head): the sum of a row's split states, in split order.
 __global__ void __launch_bounds__(256) kv4_tc_join_kernel(const KtArgs a) {
   const int lane = lane_id(), G = a.t.G, H = a.c.heads * G;
-  const long long n = (long long)a.c.rows * H;
-  const size_t stride = (size_t)a.c.heads * a.c.rows * G;
-  for (long long u = blockIdx.x * 8ll + warp_id(); u < n; u += gridDim.x * 8ll) {
-    const int row = (int)(u / H), hq = (int)(u % H);
+  const int n = a.c.rows * H;  // below 2^31 on this path
+  const size_t stride = (size_t)n;
+  for (int u = blockIdx.x * 8 + warp_id(); u < n; u += gridDim.x * 8) {
+    const int row = u / H, hq = u - row * H;
     const int b = kv4_row_seq(a.c, row);
     if (b < 0) continue;
     int first, count;
@@ -468,14 +468,16 @@ __global__ void __launch_bounds__(256) kv4_tc_join_kernel(const KtArgs a) {
     const size_t si = (size_t)(hq / G) * a.c.rows * G + (size_t)row * G + hq % G;
     const float2* ml = reinterpret_cast<const float2*>(a.t.ml_part);
     float top = -FLT_MAX;
+#pragma unroll 8
     for (int z = 0; z < a.t.splits; ++z) top = fmaxf(top, ml[z * stride + si].x);
     float sum = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int z = 0; z < a.t.splits; ++z) {
       const float2 s = ml[z * stride + si];
+      const float4 x = reinterpret_cast<const float4*>(a.t.o_part + (z * stride + si) * KT_D)[lane];
       if (s.y == 0.f) continue;  // an empty state: its O was not written
       const float f = ex2_mufu(s.x - top);
-      const float4 x = reinterpret_cast<const float4*>(a.t.o_part + (z * stride + si) * KT_D)[lane];
       sum = fmaf(s.y, f, sum);
       v.x = fmaf(x.x, f, v.x);
       v.y = fmaf(x.y, f, v.y);

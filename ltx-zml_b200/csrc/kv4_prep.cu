@@ -28,7 +28,7 @@ __device__ __forceinline__ uint32_t kv4_field(float top) {
   return (uint32_t)(f < 1 ? 1 : f > 253 ? 253 : f);
 }
 
-// CTAs [0, q_ctas): query rows, one warp per (row, head); the others: the
+// CTAs [0, q_ctas): query rows, four (row, head) a warp; the others: the
 // largest |K| and |V| that the pairs of 16 pages of one (sequence, head)
 // allow (finite groups only).
 template <int NG>
@@ -36,20 +36,38 @@ __global__ void __launch_bounds__(256) kv4_prep_kernel(const Kv4View c, const Kv
                                                        size_t ldq, int q_ctas) {
   const int lane = lane_id(), warp = warp_id(), H = c.heads * t.G;
   if ((int)blockIdx.x < q_ctas) {
-    const long long n = (long long)c.rows * H;
-    for (long long u = blockIdx.x * 8ll + warp; u < n; u += q_ctas * 8ll) {
-      const int row = (int)(u / H), h = (int)(u % H);
-      const uint2 w = __ldg(reinterpret_cast<const uint2*>(q + row * ldq + h * KV4_D + lane * 4));
-      const float x[4] = {bf16_lo(w.x), bf16_hi(w.x), bf16_lo(w.y), bf16_hi(w.y)};
-      float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+    // four (row, head) rows a warp and step; rows * H < 2^31 here
+    const int n = c.rows * H;
+    for (int u0 = ((int)blockIdx.x * 8 + warp) * 4; u0 < n; u0 += q_ctas * 32) {
+      uint2 w[4];
+      float top[4];
+      int row[4], h[4];
 #pragma unroll
-      for (int s = 1; s < 32; s <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-      const uint32_t field = kv4_field(top);
-      // the sign of the softmax scale goes with the row, so that q_scale is positive
-      const float f = t.cs == 0.f ? 0.f : copysignf(__uint_as_float(field << 23), t.cs);
-      const size_t o = (size_t)(h / t.G) * ((size_t)c.rows * t.G) + (size_t)row * t.G + h % t.G;
-      reinterpret_cast<uint2*>(t.q16)[o * 32 + lane] = make_uint2(pack_h2(x[0] * f, x[1] * f), pack_h2(x[2] * f, x[3] * f));
-      if (lane == 0) t.q_scale[o] = __uint_as_float((254u - field) << 23) * fabsf(t.cs);
+      for (int i = 0; i < 4; ++i) {
+        const int u = u0 + i < n ? u0 + i : n - 1;
+        row[i] = u / H;
+        h[i] = u - row[i] * H;
+        w[i] = __ldg(reinterpret_cast<const uint2*>(q + (size_t)row[i] * ldq + h[i] * KV4_D + lane * 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        top[i] = fmaxf(fmaxf(fabsf(bf16_lo(w[i].x)), fabsf(bf16_hi(w[i].x))), fmaxf(fabsf(bf16_lo(w[i].y)), fabsf(bf16_hi(w[i].y))));
+#pragma unroll
+      for (int s = 1; s < 32; s <<= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], s));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (u0 + i >= n) break;
+        const uint32_t field = kv4_field(top[i]);
+        // the sign of the softmax scale goes with the row, so that q_scale is positive
+        const float f = t.cs == 0.f ? 0.f : copysignf(__uint_as_float(field << 23), t.cs);
+        const int hk = h[i] / t.G;
+        const size_t o = ((size_t)hk * c.rows + row[i]) * t.G + (h[i] - hk * t.G);
+        reinterpret_cast<uint2*>(t.q16)[o * 32 + lane] = make_uint2(pack_h2(bf16_lo(w[i].x) * f, bf16_hi(w[i].x) * f),
+                                                                    pack_h2(bf16_lo(w[i].y) * f, bf16_hi(w[i].y) * f));
+        if (lane == 0) t.q_scale[o] = __uint_as_float((254u - field) << 23) * fabsf(t.cs);
+      }
     }
     return;
   }
@@ -204,7 +222,7 @@ __global__ void __launch_bounds__(256) kv4_expand_kernel(const Kv4View c, const 
 
 int kv4_prepare(const Kv4View& c, const Kv4Tc& t, const void* q, size_t ldq, int group, cudaStream_t st) {
   const int H = c.heads * t.G;
-  const long long qw = ((long long)c.rows * H + 7) / 8, most = 8ll * sm_count();
+  const long long qw = ((long long)c.rows * H + 31) / 32, most = 8ll * sm_count();
   const int q_ctas = (int)(qw < most ? qw : most);
   const long long grid = q_ctas + (long long)c.batch * c.heads * t.chunks;
   const __nv_bfloat16* qb = static_cast<const __nv_bfloat16*>(q);
