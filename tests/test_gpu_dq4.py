@@ -131,3 +131,54 @@ def test_captured_and_replayed(cuda):
         a.copy_(torch.randn(m, 512, generator=torch.Generator().manual_seed(m)).to(torch.bfloat16))
         graph.replay()
         check(out, a, wq, s)
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 64, 65536), (2, 37024, 256), (12, 224, 8320), (64, 32, 32768), (3, 128, 128)])
+def test_long_and_short_columns(cuda, M, N, K):
+    """Rows that the kernel puts in order itself and rows that it does not; K split over a cluster with a remainder."""
+    import ltxb
+    wq, s = weights(N, K, 64, torch.bfloat16, 5, cuda)
+    a = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(torch.bfloat16).to(cuda)
+    out = ltxb.dq4_gemm(a, wq, s)
+    check(out, a, wq, s)
+    assert torch.equal(out, ltxb.dq4_gemm(a, wq, s))
+
+
+def test_rows_of_unequal_size(cuda):
+    """Rows and columns of A over many powers of two, up to bf16's ends."""
+    import ltxb
+    wq, s = weights(64, 1024, 32, torch.float32, 1, cuda)
+    a = torch.randn(9, 1024, generator=torch.Generator().manual_seed(0))
+    a *= torch.exp2(torch.linspace(-100, 100, 9))[:, None]
+    a[4] *= torch.exp2(torch.linspace(-30, 30, 1024))
+    a = a.to(torch.bfloat16).to(cuda)
+    check(ltxb.dq4_gemm(a, wq, s), a, wq, s)
+    check(ltxb.dq4_gemm(a[:1], wq, s), a[:1], wq, s)
+    check(ltxb.dq4_gemm(a[8:], wq, s), a[8:], wq, s)
+
+
+def test_captured_with_its_operand_kernel(cuda):
+    """12 rows: two kernels, the second starting under the first; replayed on new rows, two streams at once."""
+    import ltxb
+    wq, s = weights(512, 4096, 128, torch.bfloat16, 1, cuda)
+    a = torch.zeros(12, 4096, dtype=torch.bfloat16, device=cuda)
+    out = torch.empty(12, 512, dtype=torch.bfloat16, device=cuda)
+    ltxb.dq4_gemm(a, wq, s, out=out)
+    graphs, outs = [], []
+    for _ in range(2):
+        o = torch.empty_like(out)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            ltxb.dq4_gemm(a, wq, s, out=o)
+        graphs.append(graph)
+        outs.append(o)
+    st = torch.cuda.Stream()
+    for i in range(4):
+        a.copy_(torch.randn(12, 4096, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16))
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        check(outs[0], a, wq, s)
+        assert torch.equal(outs[0], outs[1])

@@ -625,3 +625,142 @@ def test_capacity_far_above_the_lengths(cuda):
     cache.seq_lens.fill_(701)
     ltxb.attention_kv4(q, bound, out=out)
     assert ltxb.device_status_site() == (ltxb.EINVAL, ltxb.SITE_KV4_LEN)
+
+
+# ---------------------------------------------------------------------------
+# as they are used together, and at the edges
+# ---------------------------------------------------------------------------
+
+def test_a_decoder_layer_step_by_step(cuda):
+    """Prompt rows and then single tokens through 4-bit projections, the cache
+    and the attention, against the same steps in f64 on what each holds (the
+    projections' outputs are rounded to bf16 as the operators round them)."""
+    import ltxb
+    D, H, Hkv, group, B = 512, 4, 2, 64, 3
+    lens = [70, 5, 130]
+    g = torch.Generator(device=cuda).manual_seed(0)
+    wq = [ltxb.quantize_g4(torch.randn(n, D, generator=g, device=cuda) / D ** 0.5, group)
+          for n in ((H + 2 * Hkv) * 128, D)]
+    full = []
+    for c, s in wq:
+        code = torch.stack((c & 15, c >> 4), -1).flatten(-2).double() - 8
+        full.append(code * s.double().repeat_interleave(group, 1))
+    cache = make_cache(lens, Hkv, group, cuda, max_pages=4)
+    cache.seq_lens.zero_()
+    hist = [[], []]
+
+    def layer(x, counts):
+        n = x.shape[0]
+        cache.seq_lens.add_(torch.tensor(counts, dtype=torch.int32, device=cuda))
+        rs = starts(counts, cuda)
+        qkv = ltxb.dq4_gemm(x, *wq[0]).view(n, H + 2 * Hkv, 128)
+        q, k, v = qkv[:, :H], qkv[:, H:H + Hkv], qkv[:, H + Hkv:]
+        cache.append(k, v, row_start=rs)
+        o = ltxb.attention_kv4(q, cache, row_start=rs)
+        y = ltxb.dq4_gemm(o.view(n, H * 128), *wq[1])
+        # the same in f64 from the operators' own bf16 intermediates, one step at a time
+        want = x.double() @ full[0].T
+        err = (qkv.view(n, -1).double() - want).abs()
+        # M > 64 rounds the weights to bf16 first: six root mean squares of 2^-8
+        norm = (x.double() ** 2 @ full[0].T ** 2).sqrt()
+        assert bool((err <= 2.0 ** -8 * want.abs() + 6 * 2.0 ** -8 * norm).all())
+        at = 0
+        for b, c in enumerate(counts):
+            hist[0].append((b, k[at:at + c].clone()))
+            hist[1].append((b, v[at:at + c].clone()))
+            kk, vv = (kr.held(torch.cat([t for i, t in h if i == b]).cpu(), group) for h in hist)
+            w = kr.attention(q[at:at + c].cpu(), kk, vv, True)
+            check_many(o[at:at + c], w, q[at:at + c].cpu(), kk, vv)
+            at += c
+        want = o.view(n, -1).double() @ full[1].T
+        norm = (o.view(n, -1).double() ** 2 @ full[1].T ** 2).sqrt()
+        assert bool(((y.double() - want).abs() <= 2.0 ** -8 * want.abs() + 6 * 2.0 ** -8 * norm).all())
+        return y
+    x = torch.randn(sum(lens), D, generator=g, device=cuda).to(torch.bfloat16)
+    layer(x, lens)
+    for step in range(3):
+        layer(torch.randn(B, D, generator=g, device=cuda).to(torch.bfloat16), [1] * B)
+    assert ltxb.device_status() == ltxb.OK
+
+
+def test_many_sequences(cuda):
+    """More sequences than a CTA has threads, empty ones among them; uniform and ragged rows."""
+    import ltxb
+    B, H, Hkv, group = 300, 4, 2, 32
+    lens = [(37 * b) % 200 for b in range(B)]
+    cache, k, v = filled(lens, Hkv, group, cuda, seed=2)
+    q = torch.randn(B, H, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    out = ltxb.attention_kv4(q.to(cuda), cache)
+    again = ltxb.attention_kv4(q.to(cuda), cache, row_start=starts([1] * B, cuda))
+    assert torch.equal(out, again)
+    for b in list(range(0, B, 23)) + [B - 1]:
+        want = kr.attention(q[b:b + 1], k[b], v[b], True)
+        check(out[b:b + 1], want, float(v[b].abs().max()) if lens[b] else 0.0, f"sequence {b}")
+    assert bool((out[[b for b in range(B) if lens[b] == 0]] == 0).all())
+    assert ltxb.device_status() == ltxb.OK
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """A pool of more than 4 GB whose last pages are used."""
+    import ltxb
+    block = ltxb.lib.ltxb_kv4_block_bytes(128)
+    n = (1 << 32) // (block * 8) + 40
+    pages = torch.empty(n, 8, block, dtype=torch.uint8, device=cuda)
+    lens = [200, 90]
+    table = torch.tensor([[n - 1, 3, n - 2, n - 5], [n - 7, n - 3, 0, 1]], dtype=torch.int32, device=cuda)
+    cache = ltxb.KV4Cache.from_pages(pages, table, torch.tensor(lens, dtype=torch.int32, device=cuda), group=128)
+    k, v = rows_like((290, 8, 128), 1, cuda), rows_like((290, 8, 128), 2, cuda)
+    rs = starts(lens, cuda)
+    cache.append(k, v, row_start=rs)
+    kh, vh = kr.held(k.cpu(), 128), kr.held(v.cpu(), 128)
+    kf, vf = cache.read(290, row_start=rs, dtype=torch.float32)
+    assert torch.equal(kf.cpu(), kh.float()) and torch.equal(vf.cpu(), vh.float())
+    q = torch.randn(2, 8, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    out = ltxb.attention_kv4(q.to(cuda), cache)
+    many = torch.randn(180, 8, 128, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16)
+    out2 = ltxb.attention_kv4(many.to(cuda), cache)
+    for b, at in ((0, 0), (1, 200)):
+        kk, vv = kh[at:at + lens[b]], vh[at:at + lens[b]]
+        check(out[b:b + 1], kr.attention(q[b:b + 1], kk, vv, True), float(vv.abs().max()))
+        qb = many[90 * b:90 * b + 90]
+        check_many(out2[90 * b:90 * b + 90], kr.attention(qb, kk, vv, True), qb, kk, vv)
+
+
+def test_two_streams_at_once(cuda):
+    """Calls over two caches on two streams, each with the workspace of its own call."""
+    import ltxb
+    caches = [filled([2000, 700], 4, g, cuda, seed=i) for i, g in enumerate((32, 128))]
+    q = torch.randn(2, 8, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(cuda)
+    many = torch.randn(2 * 96, 8, 128, generator=torch.Generator().manual_seed(3)).to(torch.bfloat16).to(cuda)
+    alone = [[ltxb.attention_kv4(x, c[0]) for x in (q, many)] for c in caches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in caches]
+    got = [[], []]
+    for _ in range(4):
+        for i, (c, st) in enumerate(zip(caches, streams)):
+            with torch.cuda.stream(st):
+                got[i].append([ltxb.attention_kv4(x, c[0]) for x in (q, many)])
+    torch.cuda.synchronize()
+    for i in range(2):
+        for pair in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(pair, alone[i]))
+    # a stream given by name, not the current one
+    a = ltxb.attention_kv4(q, caches[0][0], stream=streams[1])
+    streams[1].synchronize()
+    assert torch.equal(a, alone[0][0])
+
+
+def test_infinite_and_nan_queries_stay_in_their_rows(cuda):
+    import ltxb
+    cache, k, v = filled([150], 2, 64, cuda, seed=2)
+    for n in (6, 100):
+        q = torch.randn(n, 4, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+        clean = ltxb.attention_kv4(q.to(cuda), cache)
+        bad = q.clone()
+        bad[2, 1, 5] = float("nan")
+        bad[3, 0, 7] = float("inf")
+        out = ltxb.attention_kv4(bad.to(cuda), cache)
+        assert bool(out[2, 1].isnan().all()) and bool(out[3, 0].isnan().all())
+        keep = torch.ones(n, 4, dtype=torch.bool)
+        keep[2, 1] = keep[3, 0] = False
+        assert torch.equal(out[keep.to(cuda)], clean[keep.to(cuda)])
