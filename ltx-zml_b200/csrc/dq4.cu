@@ -29,8 +29,7 @@
 // of 32: 28 us; 16 x 16,384 x 4,096: 22 us. What bounds it there is the start
 // (A's records, first tiles: 3.5 us), the instructions of a tile (the scale
 // and start value of every group and output) and the cluster's sum (3 us), no
-// longer the bytes. (Four warps of
-// 32 rows each: 27, 27, 42 and 21 us.)
+// longer the bytes. (Four warps of 32 rows each: 27, 27, 42 and 21 us.)
 //
 // More rows: the weights are expanded to bf16 in the workspace (one rounding:
 // the code and a bf16 scale have up to 11 significant bits) and multiplied by

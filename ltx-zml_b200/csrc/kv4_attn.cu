@@ -16,25 +16,32 @@
 // Scale and zero thus touch only score-sized data (per group of 32 / 64 / 128).
 //
 // A warp takes 16 tokens of a page as the M side of the MMA, so up to 8 query
-// rows (the query heads that share the K/V head, times the call's tokens)
-// cost the same as one: S^T = K Q^T, then O^T = V^T P^T with P^T transposed in
+// rows (the query heads that share the K/V head, times the call's tokens) cost
+// the same as one: S^T = K Q^T, then O^T = V^T P^T with P^T transposed in
 // registers (movmatrix). q enters as f16 after a power of two per row (its 8
-// bits stay exact down to 2^-27 of the row's largest value). p s enters as f16 scaled by a power of two that
-// follows the largest V scale seen (between 2^3 and 2^7 times p): 11
-// significant bits where bf16 would keep 8, so the result's own rounding
-// dominates. Row maxima move only when a score passes them by 2^8; sums and
-// accumulators are f32.
+// bits stay exact down to 2^-27 of the row's largest value). p s enters as f16
+// scaled by a power of two that follows the largest V scale seen (between 2^3
+// and 2^7 times p): 11 significant bits where bf16 would keep 8, so the
+// result's own rounding dominates. Row maxima move only when a score passes
+// them by 2^8; sums and accumulators are f32.
 //
 // Work is split by pages, not by sequence: all (sequence, head, row tile)
-// items laid end to end are one line of pages (each item with KA_ITEM more, what
-// starting and ending it costs: without them a batch of 64 sequences of 17 to
-// 8,192 tokens took 173 us instead of 103), each CTA takes an equal piece of it, its warps take the pages of an item in turn, and a second kernel
-// joins the items that were cut (in page order, so results do not depend on
-// timing). Lengths are read on the device only. A warp has room for one
-// (page, head) block of its own: the next page's K (codes and pairs, two bulk
-// copies) arrives while it works on V, the next V while it works on K, and no
-// barrier joins the warps until an item ends. (Two buffers each for K and V
-// gained nothing: the loads alone take 95 us of 131,009 tokens' 114.)
+// items laid end to end are one line of pages (each item with KA_ITEM more,
+// what starting and ending it costs: without them a batch of 64 sequences of 17
+// to 8,192 tokens took 173 us instead of 103), each CTA takes an equal piece of
+// it, its warps take the pages of an item in turn, and a second kernel joins
+// the items that were cut (in page order, so results do not depend on timing).
+// Lengths are read on the device only. A warp has room for one (page, head)
+// block of its own: the next page's K (codes and pairs, two bulk copies)
+// arrives while it works on V, the next V while it works on K, and no barrier
+// joins the warps until an item ends.
+//
+// Measured: 131,009 tokens x 32 heads, groups of 128 (570 MB): 116 us, 4.9 TB/s;
+// the loads alone take 95. 64 sequences of 17 to 8,192 tokens, 32 heads over 8,
+// groups of 32 (328 MB): 100 us. What bounds it is the instructions of a tile
+// (230 per 16 tokens, the ALU pipe 59 % busy) under 12 warps an SM; two buffers
+// each for K and V, or 16 warps, gained nothing. One sequence of 77 tokens: 12
+// us for both kernels, latencies from the lengths to the join.
 //
 // A token whose V group is stored as NaN, or whose page number is bad, makes
 // every row that attends to it NaN and no others: where a page holds tokens
