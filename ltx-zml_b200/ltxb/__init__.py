@@ -907,7 +907,9 @@ class KV4Cache:
     [batch, max_pages] or None (sequence b owns pages b * max_pages ..),
     `seq_lens` int32 [batch]: tokens held, which the caller moves on (the
     calls read it on the device; the rows of a call are a sequence's last
-    tokens and are counted in it already)."""
+    tokens and are counted in it already). Another tensor of the same shape
+    may be assigned to seq_lens and page_table; captured graphs go on reading
+    the one they were captured with."""
 
     def __init__(self, batch: int, max_len: int, kv_heads: int, group: int = 128, device="cuda"):
         block = int(lib.ltxb_kv4_block_bytes(int(group)))
@@ -934,7 +936,7 @@ class KV4Cache:
 
     def _bind(self, pages, page_table, seq_lens, group, max_pages, max_len):
         assert pages.is_cuda, "tensors passed to libltxb must be contiguous CUDA tensors"
-        self.pages, self.page_table, self.seq_lens = pages, page_table, seq_lens
+        self._pages, self._page_table, self._seq_lens = pages, page_table, seq_lens
         self.device, self.group = pages.device, group
         self.batch, self.kv_heads, self.max_pages = seq_lens.shape[0], pages.shape[1], max_pages
         _index_tensor(seq_lens, (self.batch,), "seq_lens", self.device)
@@ -943,6 +945,32 @@ class KV4Cache:
                        pages.shape[0], self.kv_heads, group, self.batch, max_pages, int(max_len))
         self._ref = ctypes.byref(self._c)
         self._need = {}  # workspace bytes of attention calls by (rows, H)
+
+    @property
+    def pages(self):
+        return self._pages
+
+    @property
+    def page_table(self):
+        return self._page_table
+
+    @page_table.setter
+    def page_table(self, t):
+        if t is None and self._page_table is not None:
+            raise LtxbError(EINVAL, "page_table cannot be dropped: its pages are not in the sequences' order")
+        self._c.page_table = _index_tensor(t, (self.batch, self.max_pages), "page_table", self.device)
+        self._page_table = t
+
+    @property
+    def seq_lens(self):
+        return self._seq_lens
+
+    @seq_lens.setter
+    def seq_lens(self, t):
+        if t is None:
+            raise LtxbError(EINVAL, f"seq_lens must be int32 [{self.batch}]")
+        self._c.seq_lens = _index_tensor(t, (self.batch,), "seq_lens", self.device)
+        self._seq_lens = t
 
     def _call(self, fn, stream, *args) -> None:
         if torch.cuda.current_device() == self.device.index:
@@ -1001,6 +1029,8 @@ def attention_kv4(q, cache: KV4Cache, row_start=None, causal: bool = True, gate=
             with _device(cache.device):  # its size goes by the device's number of SMs
                 need = cache._need[rows, H] = lib.ltxb_attention_kv4_workspace_bytes(cache._ref, rows, H)
         workspace = _scratch(need, cache.device, stream)
+    elif workspace.device != cache.device:
+        raise LtxbError(EINVAL, f"workspace is on {workspace.device}, the cache on {cache.device}")
     ws, ws_bytes = (None, 0) if workspace is None else (_ptr(workspace), workspace.numel())
     cache._call(lib.ltxb_attention_kv4, stream, rs, q.data_ptr(), ldq, _ptr(out), _ptr(gate), rows, H, int(causal),
                 128 ** -0.5 if scale is None else float(scale), ws, ws_bytes)

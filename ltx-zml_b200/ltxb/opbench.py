@@ -5,11 +5,19 @@ timing and for sizing profiler captures:
     PYTHONPATH=ltx-zml_b200 python -m ltxb.opbench dq_gemm --M 8192 --N 4096 --K 4096 [--unfused]
     PYTHONPATH=ltx-zml_b200 python -m ltxb.opbench gemm --M 8192 --N 4096 --K 4096
     PYTHONPATH=ltx-zml_b200 python -m ltxb.opbench block --T 8192 --reps 3 [--phases]
+    PYTHONPATH=ltx-zml_b200 python -m ltxb.opbench attention_kv4 --batch 32 --Tkv 16384 --H 8 --kv-heads 1 --group 128
+    PYTHONPATH=ltx-zml_b200 python -m ltxb.opbench kv4_append --T 8192 --kv-heads 32 --group 64
+    PYTHONPATH=ltx-zml_b200 python -m ltxb.opbench kv4_read --T 8192 --kv-heads 32 --group 64
+    PYTHONPATH=ltx-zml_b200 python -m ltxb.opbench dq4_gemm --M 8 --N 36864 --K 4096 --group 128
 
 `block` runs whole int8 blocks (BASELINE config-3 architecture: D 4096,
 32 x 128 heads, FFN 16384, S 128, int8 g128 EXT weights with bf16 scales)
 at T tokens, so every kernel of the block can be captured at a size chosen
 for the profiler (`ncu -k regex:<kernel> -s <skip> -c 1`).
+
+`attention_kv4` attends with --rows tokens per sequence (1: decoding) over
+--batch sequences of --Tkv tokens in the 4-bit cache; `kv4_append` and
+`kv4_read` move --T tokens of one sequence.
 
 Inputs are seeded N(0, 1) activations and N(0, 0.02) weights generated on the
 device; each run prints one line with the CUDA-event time per launch and the
@@ -22,7 +30,8 @@ import argparse
 
 import torch
 
-from . import attention, dq_gemm, gemm_bf16, device_status, profile_collect, profile_enable
+from . import (KV4Cache, attention, attention_kv4, device_status, dq4_gemm, dq_gemm, gemm_bf16, profile_collect,
+               profile_enable, quantize_g4)
 
 
 def _time(fn, reps: int) -> float:
@@ -37,15 +46,51 @@ def _time(fn, reps: int) -> float:
     return e0.elapsed_time(e1) / reps
 
 
+def _kv4(a, dev, g) -> int:
+    """The three calls over a 4-bit cache."""
+    tokens = a.Tkv or a.T
+    cache = KV4Cache(a.batch, tokens, a.kv_heads, a.group, device=dev)
+    k = torch.randn(tokens, a.kv_heads, 128, generator=g, device=dev).to(torch.bfloat16)
+    v = torch.randn(tokens, a.kv_heads, 128, generator=g, device=dev).to(torch.bfloat16)
+    per = 2 * (64 + 512 // a.group)  # bytes of a token and head: codes and (scale, zero) pairs of K and V
+    cache.seq_lens.fill_(tokens)
+    starts = torch.zeros(a.batch + 1, dtype=torch.int32, device=dev)
+    for b in reversed(range(a.batch)):  # the same tokens for every sequence
+        starts[b + 1:] = tokens
+        starts[: b + 1] = 0
+        cache.append(k, v, row_start=starts)
+    if a.op == "attention_kv4":
+        q = torch.randn(a.batch * a.rows, a.H, 128, generator=g, device=dev).to(torch.bfloat16)
+        out = torch.empty_like(q)
+        ms = _time(lambda: attention_kv4(q, cache, causal=False, out=out), a.reps)
+        nbytes = a.batch * tokens * a.kv_heads * per + 4 * q.numel()
+        rate = f"{4.0 * q.numel() * tokens / ms / 1e9:.1f} TFLOP/s "
+    else:
+        buf = (torch.empty_like(k), torch.empty_like(v))
+        if a.op == "kv4_append":
+            ms = _time(lambda: cache.append(k, v, row_start=starts), a.reps)
+        else:
+            ms = _time(lambda: cache.read(tokens, row_start=starts, out=buf), a.reps)
+        nbytes, rate = tokens * a.kv_heads * (512 + per), ""
+    print(f"{a.op} batch={a.batch} rows={a.rows} tokens={tokens} H={a.H} kv_heads={a.kv_heads} group={a.group}: "
+          f"{ms * 1e3:.1f} us/call {nbytes / ms / 1e6:.0f} GB/s {rate}status={device_status()}")
+    return 0
+
+
 def main(argv=None) -> int:
     ap = argparse.ArgumentParser()
-    ap.add_argument("op", choices=("attention", "dq_gemm", "gemm", "block"))
+    ap.add_argument("op", choices=("attention", "dq_gemm", "gemm", "block", "attention_kv4", "kv4_append", "kv4_read",
+                                  "dq4_gemm"))
     ap.add_argument("--T", type=int, default=8192)
     ap.add_argument("--Tkv", type=int, default=0)
     ap.add_argument("--H", type=int, default=8)
     ap.add_argument("--M", type=int, default=8192)
     ap.add_argument("--N", type=int, default=4096)
     ap.add_argument("--K", type=int, default=4096)
+    ap.add_argument("--batch", type=int, default=1)
+    ap.add_argument("--rows", type=int, default=1)
+    ap.add_argument("--kv-heads", type=int, default=8)
+    ap.add_argument("--group", type=int, default=64, choices=(32, 64, 128))
     ap.add_argument("--unfused", action="store_true")
     ap.add_argument("--reps", type=int, default=10)
     ap.add_argument("--phases", action="store_true", help="block: also print the per-phase device times")
@@ -78,6 +123,17 @@ def main(argv=None) -> int:
             ph = profile_collect(reset=True)
             print("phases (ms per block): " + " ".join(f"{k}={v[0] / max(v[2], 1):.4f}" for k, v in ph.items()))
         w.free()
+        return 0
+    if a.op in ("attention_kv4", "kv4_append", "kv4_read"):
+        return _kv4(a, dev, g)
+    if a.op == "dq4_gemm":
+        x = torch.randn(a.M, a.K, generator=g, device=dev).to(torch.bfloat16)
+        wq, sc = quantize_g4(torch.randn(a.N, a.K, generator=g, device=dev) * 0.02, a.group)
+        out = torch.empty(a.M, a.N, dtype=torch.bfloat16, device=dev)
+        ms = _time(lambda: dq4_gemm(x, wq, sc, out=out), a.reps)
+        nbytes = wq.numel() + sc.numel() * sc.element_size() + 2 * (x.numel() + out.numel())
+        print(f"dq4_gemm M={a.M} N={a.N} K={a.K} group={a.group}: {ms * 1e3:.1f} us/launch {nbytes / ms / 1e6:.0f} GB/s "
+              f"{2.0 * a.M * a.N * a.K / ms / 1e9:.1f} TFLOP/s status={device_status()}")
         return 0
     if a.op == "attention":
         tkv = a.Tkv or a.T

@@ -408,6 +408,28 @@ def test_python_refusals(cuda):
             f()
 
 
+def test_lengths_and_page_table_may_be_replaced(cuda):
+    """A length or table tensor assigned to the cache is the one that is read."""
+    import ltxb
+    cache, k, v = filled([130, 40], 2, 64, cuda, seed=4)
+    q = torch.randn(2, 4, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(cuda)
+    cache.seq_lens = cache.seq_lens - torch.tensor([70, 3], dtype=torch.int32, device=cuda)
+    got = ltxb.attention_kv4(q, cache)
+    for b, n in enumerate((60, 37)):
+        check(got[b:b + 1], kr.attention(q[b:b + 1].cpu(), k[b][:n], v[b][:n], True), float(v[b].abs().max()))
+    cache.page_table = cache.page_table.flip(0)  # the sequences change places
+    cache.seq_lens = torch.tensor([40, 130], dtype=torch.int32, device=cuda)
+    got = ltxb.attention_kv4(q, cache)
+    for b in (0, 1):
+        check(got[b:b + 1], kr.attention(q[b:b + 1].cpu(), k[1 - b], v[1 - b], True), float(v[1 - b].abs().max()))
+    for bad in (None, cache.seq_lens.long(), cache.seq_lens[:1]):
+        with pytest.raises(ltxb.LtxbError):
+            cache.seq_lens = bad
+    for bad in (None, cache.page_table[:1]):
+        with pytest.raises(ltxb.LtxbError):
+            cache.page_table = bad
+
+
 def test_deterministic_and_on_another_stream(cuda):
     import ltxb
     cache, _, _ = filled([3000, 17, 900], 2, 32, cuda, seed=3)
