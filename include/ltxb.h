@@ -557,7 +557,7 @@ int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k
  * [rows, H, 128] bf16 (q's row stride ldq elements; out contiguous), query
  * head h reading K/V head h / (H / kv_heads). causal != 0: a row sees the
  * tokens up to its own; else all of its sequence's. A row that sees nothing
- * is zero. `gate` (optional, f32 [rows, H]) multiplies each head's output.
+ * is zero; a row of q that is not finite is NaN. `gate` (optional, f32 [rows, H]) multiplies each head's output.
  * A row that attends to a token with a NaN group is NaN. Softmax, sums and
  * accumulators are f32. With fewer than 80 query rows a sequence and K/V head
  * (on average: rows * H / kv_heads / batch) the cache is read as it is and its
@@ -579,7 +579,8 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
  * scales [N, K / group] f32 or bf16, group 32, 64 or 128. K a multiple of
  * 128, N of 32; all pointers 16-byte aligned. Up to 64 rows read the weights as
  * they are, with exact products and f32 sums (the workspace holds A in the
- * order of the matrix fragments); more rows expand them to bf16 in `workspace`
+ * order of the matrix fragments; a row of A that is not finite gives NaN);
+ * more rows expand them to bf16 in `workspace`
  * (N * K * 2 bytes) for the tensor-core GEMM. Each call writes what it reads of
  * the workspace (ltxb_dq4_gemm_workspace_bytes bytes on the current device, 0
  * for a single short row); calls that may run at the same time need one each. */

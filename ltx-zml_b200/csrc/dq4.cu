@@ -473,9 +473,9 @@ __global__ void __launch_bounds__(256) dq4_expand_kernel(const uint32_t* __restr
 
 // row tiles of 8 that a launch takes at once
 static int dq4_nt(int M) { return M <= 8 ? 1 : M <= 16 ? 2 : 4; }
-// CTAs of a cluster (see above)
-// weight rows of a CTA, and the CTAs an SM holds
+// weight rows of a CTA
 static int dq4_tile(int nt) { return nt == 4 ? 256 : 128; }
+// CTAs of a cluster: the largest power of two that the SMs hold at once
 static int dq4_splits(int N, int M, int K) {
   const int nt = dq4_nt(M), tiles = (N + dq4_tile(nt) - 1) / dq4_tile(nt), chunks = (M + 8 * nt - 1) / (8 * nt);
   int S = 1;

@@ -729,7 +729,8 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
         // the item's last page on the line of pages, and the CTA that has it
         const int end = u1 - 1 + (was.pages - was.pb), head = longer * (each + 1);
         const int z = end < head ? end / (each + 1) : longer + (end - head) / each;
-        cut = make_int4(was.b, was.rt, was.h, z);
+        // (another number only if lengths changed meanwhile, or rows of sequences overlap: not followed)
+        if (z > (int)blockIdx.x && z < ctas) cut = make_int4(was.b, was.rt, was.h, z);
       }
       if (!next) a.cut[blockIdx.x] = cut;
     }

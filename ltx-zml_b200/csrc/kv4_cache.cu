@@ -66,7 +66,7 @@ __device__ __forceinline__ bool kv4_octet(const Kv4View& c, long long u, Kv4Octe
   const int len = kv4_len(c, lo), begin = len - count;  // position of row `first`; may be negative
   const int from = begin < 0 ? 0 : begin;
   const long long o = from / 8 + (u - start(lo));
-  if (u < start(lo) || o * 8 >= len) return false;
+  if (count == 0 || u < start(lo) || o * 8 >= len) return false;  // (no rows: its pages are not looked at either)
   out->b = lo;
   out->p0 = (int)(o * 8) < from ? from : (int)(o * 8);
   out->p1 = (int)(o * 8) + 8 < len ? (int)(o * 8) + 8 : len;

@@ -60,8 +60,8 @@ __global__ void __launch_bounds__(256) kv4_prep_kernel(const Kv4View c, const Kv
       for (int i = 0; i < 4; ++i) {
         if (u0 + i >= n) break;
         const uint32_t field = kv4_field(top[i]);
-        // the sign of the softmax scale goes with the row, so that q_scale is positive
-        const float f = t.cs == 0.f ? 0.f : copysignf(__uint_as_float(field << 23), t.cs);
+        // the sign of the softmax scale goes with the row, so that q_scale is positive; a row with an infinity is NaN
+        const float f = !(top[i] < INFINITY) ? NAN : t.cs == 0.f ? 0.f : copysignf(__uint_as_float(field << 23), t.cs);
         const int hk = h[i] / t.G;
         const size_t o = ((size_t)hk * c.rows + row[i]) * t.G + (h[i] - hk * t.G);
         reinterpret_cast<uint2*>(t.q16)[o * 32 + lane] = make_uint2(pack_h2(bf16_lo(w[i].x) * f, bf16_hi(w[i].x) * f),
@@ -73,6 +73,9 @@ __global__ void __launch_bounds__(256) kv4_prep_kernel(const Kv4View c, const Kv
   }
   const int u = blockIdx.x - q_ctas;
   const int chunk = u % t.chunks, bh = u / t.chunks, b = bh / c.heads, h = bh % c.heads;
+  int first, count;
+  kv4_rows(c, b, &first, &count);
+  if (count == 0) return;  // no row reads this sequence
   const int pages = (kv4_len(c, b) + KV4_PAGE - 1) / KV4_PAGE;
   float km = 0.f, vm = 0.f;
   for (int j = chunk * 16 + warp; j < pages && j < chunk * 16 + 16; j += 8) {
@@ -121,7 +124,11 @@ template <int NG>
 __global__ void __launch_bounds__(256) kv4_expand_kernel(const Kv4View c, const Kv4Tc t) {
   __shared__ float s_f[2];
   __shared__ uint32_t s_bad[2];
-  const int h = blockIdx.y, b = blockIdx.z, len = kv4_len(c, b);
+  const int h = blockIdx.y, b = blockIdx.z;
+  int first, count;
+  kv4_rows(c, b, &first, &count);
+  if (count == 0) return;
+  const int len = kv4_len(c, b);
   // the powers of two of this (sequence, head)
   if (threadIdx.x < 32) {
     const int n = ((len + KV4_PAGE - 1) / KV4_PAGE + 15) / 16;

@@ -223,13 +223,24 @@ def _stream_on(stream, dev) -> int:
 
 
 def _scratch(nbytes: int, dev, stream):
-    """Workspace of one call. It goes back to the allocator when the call has
-    returned, so a stream that is not the current one is made known to it."""
+    """Workspace of one call. For a stream other than the current one it comes
+    from that stream's pool: memory of the current stream's may still be in use
+    by what was enqueued there before."""
     if not nbytes:
         return None
-    t = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    if stream is not None:
-        t.record_stream(stream)
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=dev)
+
+
+def _result(shape, dtype, dev, stream):
+    """A result tensor, likewise; the current stream is where the caller will read it."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=dev)
+    with torch.cuda.stream(stream):
+        t = torch.empty(shape, dtype=dtype, device=dev)
+    t.record_stream(torch.cuda.current_stream(dev))
     return t
 
 
@@ -996,7 +1007,7 @@ class KV4Cache:
         if dtype not in (torch.bfloat16, torch.float32):
             raise LtxbError(EINVAL, "read: dtype must be bfloat16 or float32")
         if out is None:
-            out = torch.empty(2, rows, self.kv_heads, 128, dtype=dtype, device=self.device).unbind(0)
+            out = _result((2, rows, self.kv_heads, 128), dtype, self.device, stream).unbind(0)
             kp, vp = out[0].data_ptr(), out[1].data_ptr()
         else:
             for t in out:
@@ -1017,7 +1028,7 @@ def attention_kv4(q, cache: KV4Cache, row_start=None, causal: bool = True, gate=
     rows, H, _ = q.shape
     ldq = _row_tensor(q, H, "q", cache.device)
     if out is None:
-        out = torch.empty(rows, H, 128, dtype=torch.bfloat16, device=cache.device)
+        out = _result((rows, H, 128), torch.bfloat16, cache.device, stream)
     elif out.dtype != torch.bfloat16 or out.shape != q.shape or out.device != cache.device:
         raise LtxbError(EINVAL, "out must be bf16 like q")
     if gate is not None and (gate.dtype != torch.float32 or tuple(gate.shape) != (rows, H) or gate.device != q.device):
@@ -1097,7 +1108,7 @@ def dq4_gemm(a, wq, scales, bias=None, out=None, workspace=None, stream=None) ->
     if wq.device != dev or scales.device != dev:
         raise LtxbError(EINVAL, "dq4_gemm: tensors on different devices")
     if out is None:
-        out = torch.empty((M, N), dtype=torch.bfloat16, device=dev)
+        out = _result((M, N), torch.bfloat16, dev, stream)
     elif out.dtype != torch.bfloat16 or tuple(out.shape) != (M, N) or out.device != dev:
         raise LtxbError(EINVAL, f"dq4_gemm: out must be bf16 [{M}, {N}] on {dev}")
     with _device(dev):

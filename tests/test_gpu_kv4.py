@@ -786,3 +786,49 @@ def test_infinite_and_nan_queries_stay_in_their_rows(cuda):
         keep = torch.ones(n, 4, dtype=torch.bool)
         keep[2, 1] = keep[3, 0] = False
         assert torch.equal(out[keep.to(cuda)], clean[keep.to(cuda)])
+
+
+def test_sequences_without_rows_are_left_alone(cuda):
+    """An idle slot of a batch (no rows in the call, a length, page numbers that
+    mean nothing) is neither read nor reported, nor are rows behind the last."""
+    import ltxb
+    cache, k, v = filled([100, 61, 5], 2, 64, cuda, seed=6)
+    table = cache.page_table.clone()
+    table[1:] = 1 << 29
+    cache.page_table = table
+    before = cache.pages.clone()
+    for n in (2, 100):  # the last rows of the first sequence; the page kernel and the tcgen05 one
+        rs = starts([n, 0, 0], cuda)
+        kk, vv = cache.read(n, row_start=rs, dtype=torch.float32)
+        assert torch.equal(kk.cpu().double(), k[0][100 - n:]) and torch.equal(vv.cpu().double(), v[0][100 - n:])
+        q = torch.randn(n, 160, 128, generator=torch.Generator().manual_seed(n)).to(torch.bfloat16).to(cuda)
+        want = kr.attention(q.cpu(), k[0], v[0], True)
+        got = ltxb.attention_kv4(q[:, :160], cache, row_start=rs)
+        if n == 2:
+            check(got, want, float(v[0].abs().max()))
+        else:
+            check_many(got, want, q, k[0], v[0])
+    # written again from where it was read: the same bytes, and nothing else's
+    kb, vb = cache.read(3, row_start=starts([3, 0, 0], cuda))
+    cache.seq_lens = torch.tensor([0, 61, 5], dtype=torch.int32, device=cuda)
+    cache.append(kb[:0], vb[:0], row_start=starts([0, 0, 0], cuda))
+    cache.append(kb, vb, row_start=starts([0, 0, 0], cuda))
+    assert torch.equal(cache.pages, before)
+    assert ltxb.device_status() == ltxb.OK
+
+
+def test_infinite_queries_in_split_keys(cuda):
+    """A row whose every score is minus infinity is NaN too, in one piece and in several."""
+    import ltxb
+    k, v = rows_like((1500, 1, 128), 1, cuda), rows_like((1500, 1, 128), 2, cuda)
+    k[:, :, 7] = -50.0
+    cache = make_cache([1500], 1, 32, cuda)
+    cache.append(k, v)
+    for n in (3, 256):
+        q = torch.randn(n, 1, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(cuda)
+        clean = ltxb.attention_kv4(q, cache, causal=False)
+        q[1, 0, 7] = float("inf")
+        out = ltxb.attention_kv4(q, cache, causal=False)
+        assert bool(out[1].isnan().all())
+        keep = [i for i in range(n) if i != 1]
+        assert torch.equal(out[keep], clean[keep])
