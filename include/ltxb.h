@@ -577,13 +577,14 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
  * single rows (a token, a timestep's modulation) up. Wq [N, K / 2] bytes, the
  * even column in a byte's low half; w = (code - 8) * scale, code 0 .. 15,
  * scales [N, K / group] f32 or bf16, group 32, 64 or 128. K a multiple of
- * 128, N of 32; all pointers 16-byte aligned. Up to 64 rows read the weights as
- * they are, with exact products and f32 sums (the workspace holds A in the
- * order of the matrix fragments; a row of A that is not finite gives NaN);
- * more rows expand them to bf16 in `workspace`
- * (N * K * 2 bytes) for the tensor-core GEMM. Each call writes what it reads of
- * the workspace (ltxb_dq4_gemm_workspace_bytes bytes on the current device, 0
- * for a single short row); calls that may run at the same time need one each. */
+ * 128, N of 32; all pointers 16-byte aligned. Up to 16 rows read the
+ * weights as they are, with exact products and f32 sums (the workspace holds A
+ * in the order of the matrix fragments; a row of A that is not finite gives
+ * NaN). More rows round them once to bf16, on their way to the tensor cores, or
+ * above 1,024 rows in `workspace` (N * K * 2 bytes). Each call writes what it
+ * reads of the workspace (ltxb_dq4_gemm_workspace_bytes bytes on the current
+ * device, 0 where none is needed); calls that may run at the same time need one
+ * each. */
 uint64_t ltxb_dq4_gemm_workspace_bytes(int M, int N, int K);
 int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_dtype, int group, const void* bias,
                   void* out, int M, int N, int K, void* workspace, uint64_t workspace_bytes, void* stream);

@@ -14,10 +14,9 @@
 //   sum_k x (c - 8) s = s (sum x c - 8 sum x)
 // needs one f32 FMA per group and output. Products are exact, sums f32.
 //
-// A CTA takes 128 weight rows (256 for 17 rows of A and more) and 1 / S of K: a
-// producer warp streams [rows x 128 bytes] tiles (TMA, 256 columns) through a
-// ring, eight warps take 16 (32) rows each, both 128-column blocks of a tile
-// side by side. A's records (its values in the order of the B fragments, the
+// A CTA takes 128 weight rows and 1 / S of K: a producer warp streams [rows x
+// 128 bytes] tiles (TMA, 256 columns) through a ring, eight warps take 16 rows
+// each, both 128-column blocks of a tile side by side. A's records (its values in the order of the B fragments, the
 // groups' sums) come through the same ring from a kernel of their own, which
 // runs under this one's start; where a CTA has few values of A (DQ4_OWN), its
 // warps make them in shared memory while the ring fills. The S CTAs of a
@@ -31,9 +30,15 @@
 // and start value of every group and output) and the cluster's sum (3 us), no
 // longer the bytes. (Four warps of 32 rows each: 27, 27, 42 and 21 us.)
 //
-// More rows: the weights are expanded to bf16 in the workspace (one rounding:
-// the code and a bf16 scale have up to 11 significant bits) and multiplied by
-// the tcgen05 GEMM, as for int8 weights.
+// 17 to 1,024 rows (DQ4_TC_ROWS): the tcgen05 kernel of dq4_tc.cu, which makes
+// bf16 weights (one rounding: the code and a bf16 scale have up to 11
+// significant bits) in shared memory. The way above with four row tiles took 64
+// us for 32 x 36,864 x 4,096 (64 there), 73 for 32 x 4,096 x 16,384 (37) and 126
+// for 64 x 36,864 x 4,096 (65).
+// More rows: the same bf16 weights in the workspace, multiplied by the tcgen05
+// GEMM, as for int8 weights. There the two meet: 1,024 rows in the tcgen05 kernel
+// and 1,025 here 287 and 316 us (36,864 x 4,096), 164 and 160 (16,384 x 4,096),
+// 135 and 148 (4,096 x 16,384); at 2,048 262 and about 245 (16,384 x 4,096).
 #include <atomic>
 
 #include "common.cuh"
@@ -41,8 +46,9 @@
 
 namespace ltxb {
 
-constexpr int DQ4_STREAM_ROWS = 64;
+constexpr int DQ4_STREAM_ROWS = 16, DQ4_TC_ROWS = 1024;
 constexpr int DQ4_WARPS = 8, DQ4_THREADS = 32 * (DQ4_WARPS + 1);
+constexpr int DQ4_TILE = 128, DQ4_PER_SM = 2;  // weight rows of a CTA, CTAs an SM
 constexpr int DQ4_OWN = 2048;      // values of A (rows x columns of a CTA) that a CTA puts in order itself
 constexpr int DQ4_OWN_RECORDS = 8; // 2048 columns
 
@@ -58,7 +64,7 @@ struct Dq4Args {
   const __nv_bfloat16* bias;
   __nv_bfloat16* out;
   const __nv_bfloat16* a;
-  const uint8_t* rec;  // [M / (8 NT)][K / 256] records, or null: made from `a` by the CTA
+  const uint8_t* rec;  // [K / 256] records, or null: made from `a` by the CTA
   int M, N, K, splits;
 };
 
@@ -162,9 +168,8 @@ __global__ void __launch_bounds__(256) dq4_rows_kernel(const __nv_bfloat16* __re
   const int n = (K + 255) / 256;
   const int x = blockIdx.x * 8 + warp_id();
   if (x >= tasks) return;
-  const int m = x / n, r = x - m * n, chunk = m / (8 * NT);
-  dq4_put<NG, NT>(m < M ? A + (size_t)m * K : nullptr, r * 256, K, m - chunk * 8 * NT,
-                  rec + ((size_t)chunk * n + r) * dq4_record(NG, NT));
+  const int m = x / n, r = x - m * n;
+  dq4_put<NG, NT>(m < M ? A + (size_t)m * K : nullptr, r * 256, K, m, rec + (size_t)r * dq4_record(NG, NT));
 }
 
 __device__ __forceinline__ void dq4_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -188,10 +193,10 @@ __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
 
 template <int NG, int NT, bool OWN>
 struct Dq4Cfg {
-  static constexpr int RT = NT == 4 ? 2 : 1, ROWS = 16 * RT * DQ4_WARPS;
+  static constexpr int RT = 1, ROWS = 16 * RT * DQ4_WARPS;  // tiles of 16 weight rows a warp; weight rows of a CTA
   static constexpr int WBYTES = ROWS * 128, RECORD = dq4_record(NG, NT);
   static constexpr int STAGE = WBYTES + (OWN ? 0 : (RECORD + 1023) / 1024 * 1024);  // 1 KB: the swizzled tile's alignment
-  static constexpr int PER_SM = NT == 4 ? 1 : 2;  // CTAs an SM
+  static constexpr int PER_SM = DQ4_PER_SM;
   static constexpr int STAGES = 4;
   static constexpr int PART = 8 * NT * (ROWS + 4) * 4;
   static constexpr int SMEM = STAGES * STAGE + (OWN ? DQ4_OWN_RECORDS * RECORD : 0) + 1024 + 256;
@@ -237,7 +242,7 @@ __global__ void __launch_bounds__(DQ4_THREADS, Dq4Cfg<NG, NT, OWN>::PER_SM)
     const int n = (kb1 - kb0 + 1) / 2;  // stages of two blocks; the last may hold one
     if (lane == 0) {
       prefetch_tmap(&tmW);
-      const uint8_t* rec = OWN ? nullptr : p.rec + ((size_t)blockIdx.z * nst + kb0 / 2) * C::RECORD;
+      const uint8_t* rec = OWN ? nullptr : p.rec + (size_t)(kb0 / 2) * C::RECORD;
       auto weights = [&](int i) {  // columns past K come as zeros and are not multiplied
         const int st = i % C::STAGES;
         mbar_arrive_expect_tx(&full[st], C::WBYTES + (OWN ? 0 : C::RECORD));
@@ -416,9 +421,8 @@ __global__ void __launch_bounds__(DQ4_THREADS, Dq4Cfg<NG, NT, OWN>::PER_SM)
   else
     __syncthreads();
   const int lp = 29 - __clz(C::ROWS / S);  // this CTA's share: ROWS / S rows, four a thread
-  const int cols = p.M - (int)blockIdx.z * 8 * NT < 8 * NT ? p.M - (int)blockIdx.z * 8 * NT : 8 * NT;
-  for (int i = threadIdx.x; i < cols << lp; i += DQ4_THREADS) {
-    const int j = i >> lp, n = ((rank << lp) + (i - (j << lp))) * 4, m = blockIdx.z * 8 * NT + j;
+  for (int i = threadIdx.x; i < p.M << lp; i += DQ4_THREADS) {
+    const int j = i >> lp, n = ((rank << lp) + (i - (j << lp))) * 4, m = j;
     if (failed || n0 + n >= p.N) continue;
     const float* at = part + j * (C::ROWS + 4) + n;
     float4 v = *reinterpret_cast<const float4*>(at);
@@ -471,15 +475,13 @@ __global__ void __launch_bounds__(256) dq4_expand_kernel(const uint32_t* __restr
   for (; i < n8; i += stride) put(i, __ldg(w + i), dq4_scale(scales, scale_bf16, i >> shift));
 }
 
-// row tiles of 8 that a launch takes at once
-static int dq4_nt(int M) { return M <= 8 ? 1 : M <= 16 ? 2 : 4; }
-// weight rows of a CTA
-static int dq4_tile(int nt) { return nt == 4 ? 256 : 128; }
+// row tiles of 8 of a call
+static int dq4_nt(int M) { return M <= 8 ? 1 : 2; }
 // CTAs of a cluster: the largest power of two that the SMs hold at once
-static int dq4_splits(int N, int M, int K) {
-  const int nt = dq4_nt(M), tiles = (N + dq4_tile(nt) - 1) / dq4_tile(nt), chunks = (M + 8 * nt - 1) / (8 * nt);
+static int dq4_splits(int N, int K) {
+  const int tiles = (N + DQ4_TILE - 1) / DQ4_TILE;
   int S = 1;
-  while (S < 8 && (int64_t)tiles * chunks * S * 2 <= (nt == 4 ? 1 : 2) * sm_count() && K / 256 >= 2 * S) S *= 2;
+  while (S < 8 && (int64_t)tiles * S * 2 <= DQ4_PER_SM * sm_count() && K / 256 >= 2 * S) S *= 2;
   return S;
 }
 static bool dq4_own(int M, int K, int S) {
@@ -487,8 +489,7 @@ static bool dq4_own(int M, int K, int S) {
   return M <= 8 && cols <= DQ4_OWN_RECORDS * 256 && M * cols <= DQ4_OWN;
 }
 static uint64_t dq4_records_bytes(int M, int K) {  // for groups of 32, the largest
-  const int nt = dq4_nt(M), chunks = (M + 8 * nt - 1) / (8 * nt);
-  return (uint64_t)chunks * ((K + 255) / 256) * dq4_record(4, nt);
+  return (uint64_t)((K + 255) / 256) * dq4_record(4, dq4_nt(M));
 }
 
 template <int NG, int NT, bool BF, bool OWN>
@@ -503,12 +504,12 @@ static int dq4_launch(const void* Wq, Dq4Args p, uint8_t* ws, cudaStream_t st) {
     if (e != cudaSuccess) return set_cuda_error(e, "dq4_gemm: cudaFuncSetAttribute");
     attr[dev].store(true, std::memory_order_release);
   }
-  const int chunks = (p.M + 8 * NT - 1) / (8 * NT), tiles = (p.N + C::ROWS - 1) / C::ROWS;
+  const int tiles = (p.N + C::ROWS - 1) / C::ROWS;
   CUtensorMap tm;
   if (int rc = make_tmap_2d(&tm, Wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, p.K / 2, p.N, p.K / 2, 128, C::ROWS, CU_TENSOR_MAP_SWIZZLE_128B))
     return rc;
   cudaError_t e;
-  const int tasks = chunks * 8 * NT * ((p.K + 255) / 256);
+  const int tasks = 8 * NT * ((p.K + 255) / 256);
   if (!OWN) {
     p.rec = ws;
     dq4_rows_kernel<NG, NT><<<(tasks + 7) / 8, 256, 0, st>>>(p.a, p.M, p.K, tasks, ws);
@@ -517,7 +518,7 @@ static int dq4_launch(const void* Wq, Dq4Args p, uint8_t* ws, cudaStream_t st) {
     if (e != cudaSuccess) return set_cuda_error(e, "dq4_gemm rows");
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(tiles, p.splits, chunks);
+  cfg.gridDim = dim3(tiles, p.splits);
   cfg.blockDim = dim3(DQ4_THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
@@ -541,11 +542,10 @@ template <int NG, bool BF>
 static int dq4_stream(const void* Wq, Dq4Args p, void* workspace, cudaStream_t st) {
   const int nt = dq4_nt(p.M);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.splits = dq4_splits(p.N, p.M, p.K);
+  p.splits = dq4_splits(p.N, p.K);
   if (nt == 1)
     return dq4_own(p.M, p.K, p.splits) ? dq4_launch<NG, 1, BF, true>(Wq, p, ws, st) : dq4_launch<NG, 1, BF, false>(Wq, p, ws, st);
-  if (nt == 2) return dq4_launch<NG, 2, BF, false>(Wq, p, ws, st);
-  return dq4_launch<NG, 4, BF, false>(Wq, p, ws, st);
+  return dq4_launch<NG, 2, BF, false>(Wq, p, ws, st);
 }
 
 }  // namespace ltxb
@@ -556,8 +556,9 @@ extern "C" {
 
 uint64_t ltxb_dq4_gemm_workspace_bytes(int M, int N, int K) {
   if (M <= 0 || N <= 0 || K < 128) return 0;
-  if (M > DQ4_STREAM_ROWS) return (uint64_t)N * K * 2;
-  return dq4_own(M, K, dq4_splits(N, M, K)) ? 0 : dq4_records_bytes(M, K);
+  if (M > DQ4_TC_ROWS) return (uint64_t)N * K * 2;
+  if (M > DQ4_STREAM_ROWS) return 0;
+  return dq4_own(M, K, dq4_splits(N, K)) ? 0 : dq4_records_bytes(M, K);
 }
 
 int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_dtype, int group, const void* bias,
@@ -579,7 +580,9 @@ int ltxb_dq4_gemm(const void* A, const void* Wq, const void* scales, int scale_d
     return set_error(LTXB_EINVAL, "dq4_gemm: workspace of %llu bytes is smaller than the %llu required",
                      (unsigned long long)workspace_bytes, (unsigned long long)need);
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return set_error(LTXB_EINVAL, "dq4_gemm: workspace must be 16-byte aligned");
-  if (M > DQ4_STREAM_ROWS) {
+  if (M > DQ4_STREAM_ROWS && M <= DQ4_TC_ROWS)
+    return dq4_gemm_tc(A, Wq, scales, sb, group, bias, out, M, N, K, st);
+  if (M > DQ4_TC_ROWS) {
     GemmArgs g{};
     g.A = A;
     g.lda = K;

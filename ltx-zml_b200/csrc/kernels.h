@@ -40,6 +40,10 @@ struct Phase {
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem_bytes, int cols, int rows,
                  int ld, int box_cols, int box_rows, CUtensorMapSwizzle swz);
 
+// ---- 4-bit weights and tens to hundreds of rows (dq4_tc.cu) ----
+int dq4_gemm_tc(const void* A, const void* Wq, const void* scales, int scale_bf16, int group, const void* bias, void* out,
+                int M, int N, int K, cudaStream_t st);
+
 // ---- tcgen05 GEMM ----
 enum Epi : int {
   EPI_BF16 = 0,          // out bf16 = acc (+ bias)

@@ -1,8 +1,8 @@
 """GPU tests of the linear with 4-bit weights (ltxb_dq4_gemm) against float64.
 
 Tolerances. Few rows: exact products, f32 sums, one output rounding: at most
-2^-8 |want|, plus f32 accumulation, far below 2^-16 of sum |x w|. More rows:
-the weights are rounded to bf16 first, 2^-8 each, so the sum is off by at most
+2^-8 |want|, plus f32 accumulation, far below 2^-16 of sum |x w|. More than 16
+rows: the weights are rounded to bf16 first, 2^-8 each, so the sum is off by at most
 2^-8 sum |x w| more; where the roundings are independent that is a root mean
 square of 2^-8 |x| |w| (2-norms), and six of those bound every element here."""
 
@@ -36,7 +36,7 @@ def exact(a, wq, scales, bias=None):
 def check(got, a, wq, scales, bias=None):
     want, total, norm = exact(a, wq, scales, bias)
     bound = 2.0 ** -8 * want.abs() + 2.0 ** -16 * total
-    if a.shape[0] > 64:
+    if a.shape[0] > 16:
         bound += 6 * 2.0 ** -8 * norm
     err = (got.double().cpu() - want).abs()
     assert bool((err <= bound).all()), float((err / bound).max())
@@ -52,6 +52,28 @@ def test_dq4_gemm(cuda, M, N, K, group, scale_dtype):
     bias = torch.randn(N, generator=g).to(torch.bfloat16).to(cuda)
     check(ltxb.dq4_gemm(a, wq, s), a, wq, s)
     check(ltxb.dq4_gemm(a, wq, s, bias=bias), a, wq, s, bias)
+    assert ltxb.device_status() == ltxb.OK
+
+
+# Each side of the borders between the three ways: rows in one and several
+# chunks, weight rows and columns with a remainder, K split over a cluster.
+BORDERS = [(16, 160, 640), (17, 160, 640), (48, 4096, 8320), (255, 32, 2176), (256, 384, 1152), (257, 160, 128),
+           (700, 288, 16512), (1024, 96, 512), (1025, 96, 512)]
+
+
+@pytest.mark.parametrize("group,scale_dtype", [(128, torch.float32), (64, torch.bfloat16), (32, torch.float32),
+                                               (32, torch.bfloat16)])
+@pytest.mark.parametrize("M,N,K", BORDERS)
+def test_borders_between_the_kernels(cuda, M, N, K, group, scale_dtype):
+    import ltxb
+    wq, s = weights(N, K, group, scale_dtype, M, cuda)
+    a = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(torch.bfloat16).to(cuda)
+    bias = torch.randn(N, generator=torch.Generator().manual_seed(N)).to(torch.bfloat16).to(cuda)
+    guard = torch.full((M + 2, N), 7.0, dtype=torch.bfloat16, device=cuda)
+    out = ltxb.dq4_gemm(a, wq, s, bias=bias, out=guard[1:M + 1])
+    check(out, a, wq, s, bias)
+    assert bool((guard[0] == 7).all()) and bool((guard[M + 1] == 7).all())
+    assert torch.equal(out, ltxb.dq4_gemm(a, wq, s, bias=bias))
     assert ltxb.device_status() == ltxb.OK
 
 
@@ -80,10 +102,15 @@ def test_rows_do_not_depend_on_their_neighbours(cuda):
     b[5, 7] = float("inf")
     t = s.clone()
     t[20, 2] = float("nan")
+    many = ltxb.dq4_gemm(b.repeat(3, 1), wq, t)  # 36 rows: the tcgen05 kernel
+    plain = ltxb.dq4_gemm(a.repeat(3, 1), wq, s)
     out = ltxb.dq4_gemm(b, wq, t)
     rows = [r for r in range(12) if r not in (3, 5)]
     cols = [c for c in range(64) if c != 20]
     assert torch.equal(out[rows][:, cols], clean[rows][:, cols])
+    keep = [r for r in range(36) if r % 12 not in (3, 5)]
+    assert torch.equal(many[keep][:, cols], plain[keep][:, cols]) and bool(many[:, 20].isnan().all())
+    assert bool(many[3].isnan().all()) and not bool(many[5].isfinite().any())
     assert bool(out[3].isnan().all()) and not bool(out[5].isfinite().any()) and bool(out[:, 20].isnan().all())
 
 
@@ -111,7 +138,7 @@ def test_refusals(cuda):
               lambda: ltxb.dq4_gemm(a, wq, s[:, :3].contiguous()), lambda: ltxb.dq4_gemm(a, wq, s[:, :1].contiguous()),
               lambda: ltxb.dq4_gemm(a, wq[:48], s[:48]), lambda: ltxb.dq4_gemm(a, wq, s, bias=s[:, 0]),
               lambda: ltxb.dq4_gemm(a, wq.cpu(), s), lambda: ltxb.dq4_gemm(a, wq, s, out=a),
-              lambda: ltxb.dq4_gemm(a.repeat(50, 1), wq, s, workspace=torch.empty(16, dtype=torch.uint8, device=cuda))):
+              lambda: ltxb.dq4_gemm(a.repeat(8, 1), wq, s, workspace=torch.empty(16, dtype=torch.uint8, device=cuda))):
         with pytest.raises(ltxb.LtxbError):
             f()
     assert ltxb.launch_count() == n0

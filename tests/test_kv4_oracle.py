@@ -131,10 +131,11 @@ def test_bad_4bit_linear_calls_are_refused():
         return f(A, W, S, dt, group, bias, out, M, N, K, ws, wb, None)
     refused = [call(dt=ltxb.DT_I8), call(group=16), call(group=256), call(M=-1), call(N=0), call(N=48), call(K=64),
                call(K=0), call(A=at + 2), call(A=None), call(W=at + 8), call(W=None), call(S=at + 4), call(S=None),
-               call(out=at + 2), call(out=None), call(bias=at + 2), call(M=1000, wb=100), call(M=1000, ws=None),
-               call(M=1000, ws=at + 8), call(M=9, ws=None), call(M=9, wb=100), call(M=9, ws=at + 8)]
+               call(out=at + 2), call(out=None), call(bias=at + 2), call(M=1025, wb=100), call(M=1025, ws=None),
+               call(M=1025, ws=at + 8), call(M=9, ws=None), call(M=9, wb=100), call(M=9, ws=at + 8)]
     assert refused == [ltxb.EINVAL] * len(refused)
     assert call(M=0, A=None, W=None) == ltxb.OK
     assert ltxb.launch_count() == n0
     assert ltxb.lib.ltxb_dq4_gemm_workspace_bytes(1, 32, 128) == 0
-    assert ltxb.lib.ltxb_dq4_gemm_workspace_bytes(1000, 32, 128) == 32 * 128 * 2
+    assert ltxb.lib.ltxb_dq4_gemm_workspace_bytes(1025, 32, 128) == 32 * 128 * 2
+    assert ltxb.lib.ltxb_dq4_gemm_workspace_bytes(1024, 32, 128) == 0
