@@ -33,8 +33,8 @@
 // 17 to 1,024 rows (DQ4_TC_ROWS): the tcgen05 kernel of dq4_tc.cu, which makes
 // bf16 weights (one rounding: the code and a bf16 scale have up to 11
 // significant bits) in shared memory. The way above with four row tiles took 64
-// us for 32 x 36,864 x 4,096 (64 there), 73 for 32 x 4,096 x 16,384 (37) and 126
-// for 64 x 36,864 x 4,096 (65).
+// us for 32 x 36,864 x 4,096 (58 there), 73 for 32 x 4,096 x 16,384 (35) and 126
+// for 64 x 36,864 x 4,096 (59).
 // More rows: the same bf16 weights in the workspace, multiplied by the tcgen05
 // GEMM, as for int8 weights. There the two meet: 1,024 rows in the tcgen05 kernel
 // and 1,025 here 287 and 316 us (36,864 x 4,096), 164 and 160 (16,384 x 4,096),

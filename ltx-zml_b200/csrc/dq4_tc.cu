@@ -5,7 +5,7 @@
 //
 // D^T = W A^T: 128 weight rows are the M side of the MMA and up to 256 rows of A
 // the N side, so a few dozen rows do not leave the tensor core idle on padding.
-// Per 64 columns of K, eight warps take a [128 x 64] tile of codes from a TMA
+// Per step of 64 or 128 columns of K, eight warps take a tile of codes from a TMA
 // ring (256 columns a stage), put code - 8 (exact in bf16: 128 + code is a bit
 // pattern) times the scale (one rounding; an f32 scale as two bf16 parts) into
 // a swizzled tile, and one thread issues the MMAs against A's tile, which comes
@@ -14,12 +14,13 @@
 // f32 sums in TMEM. Where tiles are few, the CTAs of a cluster take parts of K
 // and add their f32 sums in rank order through distributed shared memory.
 //
-// Measured (groups of 64): 17 to 64 rows x 16,384 x 4,096 37 to 39 us, 128 rows
-// 41, 256 rows 47 (730 TFLOP/s), 1,001 rows 148 (910). What bounds it below
-// 200 rows is the hand-over of a block of 64 columns (a barrier, four MMAs, a
-// commit: 0.38 us, whatever the rows): taking the codes unconverted saves 4 % of
-// the time, a second group of unpacking warps 7 %, four accumulators in turn
-// nothing. Above, the MMAs.
+// Measured (groups of 64): 17 to 64 rows x 16,384 x 4,096 33 us, 128 rows 35, 256
+// rows 43 to 47 (760 TFLOP/s), 1,001 rows 146 (920). What bounds it below 200
+// rows is the unpacking and the hand-over of a step (1.3 us per 256 columns,
+// whatever the rows); above, the MMAs (2 us per 256 columns of 256 rows), and
+// each CTA's start and end, about 10 us. Steps of 64 columns: taking the codes
+// unconverted saved 4 %, a second group of unpacking warps 7 %; four
+// accumulators in turn gained nothing.
 #include <atomic>
 
 #include "attn_math.cuh"
@@ -28,7 +29,7 @@
 
 namespace ltxb {
 
-constexpr int DT_GROUPS = 2, DT_WARPS = 8 * DT_GROUPS;  // unpacking: groups of 8 warps take blocks of 64 columns in turn
+constexpr int DT_GROUPS = 2, DT_WARPS = 8 * DT_GROUPS;  // unpacking: groups of 8 warps take steps in turn
 constexpr int DT_SCALERS = 4;  // warps that fetch scales
 constexpr int DT_THREADS = 32 * (DT_WARPS + 3 + DT_SCALERS);
 constexpr int DT_ROWS = 128;  // weight rows of a CTA
@@ -44,7 +45,7 @@ struct DtArgs {
   __nv_bfloat16* out;
   int M, N, K, splits;
   int mpad;    // rows of A of a CTA, a multiple of 16
-  int wslots, aslots;  // stages of codes and bf16 tiles; tiles of A
+  int wslots, dslots, aslots;  // ring slots: stages of codes, steps of bf16 weights, steps of A
   int shift;   // log2(group / 32)
   int sbytes;  // of a stage's scales
   uint32_t tmem_cols;
@@ -103,14 +104,15 @@ __device__ __forceinline__ float4 dt_ld_cluster4(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-template <bool BF>
+// STEP: blocks of 64 columns that are handed over together.
+template <bool BF, int STEP>
 __global__ void __launch_bounds__(DT_THREADS, 1)
     dq4_tc_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmA, const DtArgs p) {
   extern __shared__ uint8_t dt_raw[];
   uint8_t* wring = dt_raw + (-smem_u32(dt_raw) & 1023u);
   uint8_t* tiles = wring + p.wslots * DT_WBYTES;  // bf16 weights
-  uint8_t* aring = tiles + p.wslots * DT_TILE;
-  const int abytes = p.mpad * 128;
+  uint8_t* aring = tiles + p.dslots * STEP * DT_TILE;
+  const int ablock = p.mpad * 128, abytes = STEP * ablock;
   uint8_t* sring = aring + p.aslots * abytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(wring + DT_SMEM);
   uint64_t *wfull = bars, *wempty = bars + 4, *dfull = bars + 8, *done = bars + 12, *afull = bars + 14,
@@ -118,9 +120,10 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   const int warp = warp_id(), lane = lane_id();
   const int n0 = blockIdx.x * DT_ROWS, rank = blockIdx.y, S = p.splits, m0 = blockIdx.z * p.mpad;
-  // stages of 256 columns [s0, s1), blocks of 64 columns [kb0, kb1)
+  // stages of 256 columns [s0, s1), steps [kb0, kb1)
+  constexpr int SPS = 4 / STEP, COLS = 64 * STEP;
   const int nst = (p.K + 255) / 256, s0 = (int)((long long)rank * nst / S), s1 = (int)((long long)(rank + 1) * nst / S);
-  const int kb0 = 4 * s0, kb1 = 4 * s1 < p.K / 64 ? 4 * s1 : p.K / 64;
+  const int kb0 = SPS * s0, kb1 = SPS * s1 < p.K / COLS ? SPS * s1 : p.K / COLS;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 4; ++i) {
@@ -145,36 +148,42 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   if (warp < DT_WARPS) {
     // ---------------- codes -> bf16: thread (group, row, half) takes 32 of 64 columns ----------------
     const int row = threadIdx.x & 127, half = (threadIdx.x >> 7) & 1, grp = warp >> 3;
-    constexpr int BLOCKS = 4 / DT_GROUPS;  // of a stage
-    int ds = grp, it = grp;  // slot and number of the block
+    int ds = grp, it = grp;  // slot and number of the step
     uint32_t wph = 0;
     for (int s = s0, ws = 0; s < s1 && ok; ++s) {
       ok = warp_wait(&wfull[ws], wph, 0x331);
       if (!ok) break;
       const uint8_t* srow = sring + ws * p.sbytes + row * (BF ? 4 : 8);
       const uint8_t* wrow = wring + ws * DT_WBYTES + row * 128;
-      const int nk = kb1 - 4 * s < 4 ? kb1 - 4 * s : 4;
+      const int nk = kb1 - SPS * s < SPS ? kb1 - SPS * s : SPS;
 #pragma unroll
-      for (int i = 0; i < BLOCKS; ++i) {
+      for (int i = 0; i < SPS / DT_GROUPS; ++i) {
         const int k = i * DT_GROUPS + grp;
         if (k >= nk) break;
-        const uint4 w = *reinterpret_cast<const uint4*>(wrow + (((2 * k + half) ^ (row & 7)) << 4));
-        const uint8_t* sp = srow + ((2 * k + half) >> p.shift) * (DT_SROW * (BF ? 4 : 8));
-        const uint32_t hi = *reinterpret_cast<const uint32_t*>(sp), lo = BF ? 0u : *reinterpret_cast<const uint32_t*>(sp + 4);
-        const uint4 r0 = dt_weights<BF>(w.x, hi, lo), r1 = dt_weights<BF>(w.y, hi, lo), r2 = dt_weights<BF>(w.z, hi, lo),
-                    r3 = dt_weights<BF>(w.w, hi, lo);
-        if (it >= p.wslots) ok = warp_wait(&mdone[(it - p.wslots) % DT_MAXST], ((it - p.wslots) / DT_MAXST) & 1, 0x332);
+        uint4 r[STEP][4];
+#pragma unroll
+        for (int t = 0; t < STEP; ++t) {
+          const int c = 2 * (k * STEP + t) + half;  // of the stage's eight blocks of 32 columns
+          const uint4 w = *reinterpret_cast<const uint4*>(wrow + ((c ^ (row & 7)) << 4));
+          const uint8_t* sp = srow + (c >> p.shift) * (DT_SROW * (BF ? 4 : 8));
+          const uint32_t hi = *reinterpret_cast<const uint32_t*>(sp), lo = BF ? 0u : *reinterpret_cast<const uint32_t*>(sp + 4);
+          r[t][0] = dt_weights<BF>(w.x, hi, lo);
+          r[t][1] = dt_weights<BF>(w.y, hi, lo);
+          r[t][2] = dt_weights<BF>(w.z, hi, lo);
+          r[t][3] = dt_weights<BF>(w.w, hi, lo);
+        }
+        if (it >= p.dslots) ok = warp_wait(&mdone[(it - p.dslots) % DT_MAXST], ((it - p.dslots) / DT_MAXST) & 1, 0x332);
         if (!ok) break;
-        uint8_t* d = tiles + ds * DT_TILE + row * 128;
-        *reinterpret_cast<uint4*>(d + (((half * 4 + 0) ^ (row & 7)) << 4)) = r0;
-        *reinterpret_cast<uint4*>(d + (((half * 4 + 1) ^ (row & 7)) << 4)) = r1;
-        *reinterpret_cast<uint4*>(d + (((half * 4 + 2) ^ (row & 7)) << 4)) = r2;
-        *reinterpret_cast<uint4*>(d + (((half * 4 + 3) ^ (row & 7)) << 4)) = r3;
+        uint8_t* d = tiles + ds * STEP * DT_TILE + row * 128;
+#pragma unroll
+        for (int t = 0; t < STEP; ++t)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(d + t * DT_TILE + (((half * 4 + j) ^ (row & 7)) << 4)) = r[t][j];
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&dfull[ds]);
         it += DT_GROUPS;
-        if ((ds += DT_GROUPS) >= p.wslots) ds -= p.wslots;
+        if ((ds += DT_GROUPS) >= p.dslots) ds -= p.dslots;
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&wempty[ws]);
@@ -205,15 +214,17 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
       if (ok) ok = warp_wait(&dfull[ds], ph, 0x336);
       if (!ok) break;
       tc_fence_after();
-      const uint32_t dw = w0 + ds * (DT_TILE >> 4), da = a0 + as * (abytes >> 4);
+      const uint32_t dw = w0 + ds * (STEP * DT_TILE >> 4), da = a0 + as * (abytes >> 4);
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_ss_lo(tmem, dw + 2 * k, da + 2 * k, idesc, (i | k) != 0);
+        for (int k = 0; k < 4 * STEP; ++k)
+          mma_ss_lo(tmem, dw + (k >> 2) * (DT_TILE >> 4) + 2 * (k & 3), da + (k >> 2) * (ablock >> 4) + 2 * (k & 3), idesc,
+                    (i | k) != 0);
         umma_commit(&mdone[i % DT_MAXST]);
         if (i == kb1 - kb0 - 1) umma_commit(done);
       }
       __syncwarp();
-      if (++ds == p.wslots) ds = 0, ph ^= 1;
+      if (++ds == p.dslots) ds = 0, ph ^= 1;
       if (++as == p.aslots) as = 0, aph ^= 1;
     }
   } else if (warp == DT_WARPS + 2) {
@@ -226,7 +237,9 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
         if (before >= 0) ok = mbar_wait(&mdone[before % DT_MAXST], (before / DT_MAXST) & 1, 0x337);
         if (!ok) break;
         mbar_arrive_expect_tx(&afull[as], abytes);
-        tma_load_2d(aring + as * abytes, &tmA, &afull[as], (kb0 + i) * 64, m0);  // rows past M come as zeros
+#pragma unroll
+        for (int t = 0; t < STEP; ++t)  // rows past M come as zeros
+          tma_load_2d(aring + as * abytes + t * ablock, &tmA, &afull[as], (kb0 + i) * COLS + t * 64, m0);
         if (++as == (uint32_t)p.aslots) as = 0;
       }
     }
@@ -344,11 +357,11 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   dt_cluster_sync();  // the others have read this CTA's sums
 }
 
-// CTAs of a cluster: waves of CTAs times their stages (1.4 us and 0.7 more with
+// CTAs of a cluster: waves of CTAs times their stages (1.3 us and 0.7 more with
 // 256 rows) and about 6 us for starting and ending, with clusters 2 more.
 static int dt_splits(int units, int nst, int mpad) {
   const int sms = sm_count();
-  const double per = 1.4 + 0.7 * mpad / 256;
+  const double per = 1.3 + 0.7 * mpad / 256;
   int best = 1;
   double best_t = 0;
   for (int s = 1; s <= 8 && 2 * s <= nst; s *= 2) {
@@ -370,24 +383,31 @@ int dq4_gemm_tc(const void* A, const void* Wq, const void* scales, int scale_bf1
   p.shift = group == 128 ? 2 : group == 64 ? 1 : 0;
   const int chunks = (M + DT_MAXM - 1) / DT_MAXM, tiles = (N + DT_ROWS - 1) / DT_ROWS;
   p.mpad = ((M + chunks - 1) / chunks + 15) / 16 * 16;
-  p.wslots = p.mpad <= 128 ? 4 : 3;
+  // Steps of 128 columns as long as two of A's fit beside them: a hand-over costs
+  // nearly as much for 128 columns as for 64 (128 rows x 16,384 x 4,096: 35 us
+  // instead of 41, 36,864 x 4,096: 62 instead of 70).
+  const bool two = p.mpad <= 128;
+  p.wslots = 3;
+  p.dslots = two ? 2 : 3;
+  const int step = two ? 2 : 1;
   p.sbytes = (8 >> p.shift) * DT_SROW * (scale_bf16 ? 4 : 8);
-  const int fit = (DT_SMEM - p.wslots * (DT_WBYTES + DT_TILE + p.sbytes)) / (p.mpad * 128);  // 3 or more
+  const int fit = (DT_SMEM - p.wslots * (DT_WBYTES + p.sbytes) - p.dslots * step * DT_TILE) / (step * p.mpad * 128);  // 2 or more
   p.aslots = fit < DT_MAXST ? fit : DT_MAXST;
   p.splits = dt_splits(tiles * chunks, (K + 255) / 256, p.mpad);
   p.tmem_cols = 32;
   while ((int)p.tmem_cols < p.mpad) p.tmem_cols *= 2;
   constexpr int bytes = DT_SMEM + DT_BARS + 1024;
-  auto kern = scale_bf16 ? dq4_tc_kernel<true> : dq4_tc_kernel<false>;
-  static std::atomic<bool> attr[2][kMaxDevices];
+  const int which = 2 * scale_bf16 + two;
+  auto kern = which == 0 ? dq4_tc_kernel<false, 1> : which == 1 ? dq4_tc_kernel<false, 2> : which == 2 ? dq4_tc_kernel<true, 1> : dq4_tc_kernel<true, 2>;
+  static std::atomic<bool> attr[4][kMaxDevices];
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= kMaxDevices) return set_error(LTXB_EINVAL, "dq4_gemm: device %d out of range", dev);
   cudaError_t e;
-  if (!attr[scale_bf16][dev].load(std::memory_order_acquire)) {
+  if (!attr[which][dev].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return set_cuda_error(e, "dq4_gemm: cudaFuncSetAttribute");
-    attr[scale_bf16][dev].store(true, std::memory_order_release);
+    attr[which][dev].store(true, std::memory_order_release);
   }
   CUtensorMap tw, ta;
   if (int rc = make_tmap_2d(&tw, Wq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, K / 2, N, K / 2, 128, DT_ROWS, CU_TENSOR_MAP_SWIZZLE_128B))
