@@ -28,7 +28,7 @@
 // Work is split by pages, not by sequence: all (sequence, head, row tile)
 // items laid end to end are one line of pages (each item with KA_ITEM more,
 // what starting and ending it costs: without them a batch of 64 sequences of 17
-// to 8,192 tokens took 173 us instead of 103), each CTA takes an equal piece of
+// to 8,192 tokens took 173 us instead of 100), each CTA takes an equal piece of
 // it, its warps take the pages of an item in turn, and a second kernel joins
 // the items that were cut (in page order, so results do not depend on timing).
 // Lengths are read on the device only. A warp has room for one (page, head)
@@ -36,9 +36,9 @@
 // arrives while it works on V, the next V while it works on K, and no barrier
 // joins the warps until an item ends.
 //
-// Measured: 131,009 tokens x 32 heads, groups of 128 (570 MB): 116 us, 4.9 TB/s;
+// Measured: 131,009 tokens x 32 heads, groups of 128 (570 MB): 117 us, 4.9 TB/s;
 // the loads alone take 95. 64 sequences of 17 to 8,192 tokens, 32 heads over 8,
-// groups of 32 (328 MB): 100 us. What bounds it is the instructions of a tile
+// groups of 32 (328 MB): 93 us. 8 of 900 to 2,500, 16 rows each: 26 us. What bounds it is the instructions of a tile
 // (230 per 16 tokens, the ALU pipe 59 % busy) under 12 warps an SM; two buffers
 // each for K and V, or 16 warps, gained nothing. One sequence of 77 tokens: 12
 // us for both kernels, latencies from the lengths to the join.

@@ -209,3 +209,25 @@ def test_captured_with_its_operand_kernel(cuda):
         torch.cuda.synchronize()
         check(outs[0], a, wq, s)
         assert torch.equal(outs[0], outs[1])
+
+
+def test_two_streams_at_once(cuda):
+    """Calls of the tcgen05 kernel side by side, with K split over clusters and without."""
+    import ltxb
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    jobs, alone = [], []
+    for i, (m, n, k) in enumerate(((40, 2048, 8192), (200, 20480, 1024))):
+        wq, s = weights(n, k, 64, torch.bfloat16, i, cuda)
+        a = torch.randn(m, k, generator=torch.Generator().manual_seed(i)).to(torch.bfloat16).to(cuda)
+        jobs.append((a, wq, s))
+        alone.append(ltxb.dq4_gemm(a, wq, s))
+        check(alone[i], a, wq, s)
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, st in enumerate(streams):
+            got[i].append(ltxb.dq4_gemm(*jobs[i], stream=st))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(o, alone[i]) for o in got[i])
+    assert ltxb.device_status() == ltxb.OK
