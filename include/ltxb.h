@@ -559,7 +559,8 @@ int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k
  * tokens up to its own; else all of its sequence's. A row that sees nothing
  * is zero; a row of q that is not finite is NaN. `gate` (optional, f32 [rows, H]) multiplies each head's output.
  * A row that attends to a token with a NaN group is NaN. Softmax, sums and
- * accumulators are f32. With fewer than 80 query rows a sequence and K/V head
+ * accumulators are f32. (Sums hold p up to 2^8 times V: |V| below 2^100 cannot
+ * overflow them.) With fewer than 80 query rows a sequence and K/V head
  * (on average: rows * H / kv_heads / batch) the cache is read as it is and its
  * codes enter the products exactly; with more, K and V are laid out in the
  * workspace as f16 (one rounding of 2^-12) for the tcgen05 kernel, which takes
