@@ -38,17 +38,12 @@ PAGE = 64
 HD = 128
 
 
-_lib = None
-
-
 def _ltxb():
-    """The package, imported at its first use."""
-    global _lib
-    if _lib is None:
-        sys.path.insert(0, str(pathlib.Path(__file__).resolve().parents[1] / "ltx-zml_b200"))
-        import ltxb
-        _lib = ltxb
-    return _lib
+    p = str(pathlib.Path(__file__).resolve().parents[1] / "ltx-zml_b200")
+    if p not in sys.path:
+        sys.path.insert(0, p)
+    import ltxb
+    return ltxb
 
 
 # ---------------------------------------------------------------------------
