@@ -178,8 +178,10 @@ __device__ __forceinline__ void dq4_bulk(void* dst, const void* src, uint32_t by
                "l"(src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
+// (Not the .aligned form: that one needs a warp's lanes to come together, and
+// they come from loops of unequal length.)
 __device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ float4 ld_cluster4(uint32_t addr, uint32_t rank) {
   float4 v;
@@ -290,12 +292,14 @@ __global__ void __launch_bounds__(DQ4_THREADS, Dq4Cfg<NG, NT, OWN>::PER_SM)
       const int n = (nb + 1) / 2;
       for (int i = threadIdx.x; i < n * C::RECORD / 16; i += DQ4_WARPS * 32)  // rows past M stay zeros
         reinterpret_cast<uint4*>(recs)[i] = make_uint4(0, 0, 0, 0);
+      __syncwarp();  // (the barrier takes whole warps; the loop's last step only some of their lanes)
       named_bar(1, DQ4_WARPS * 32);
 #pragma unroll 1
       for (int x = warp; x < n * p.M; x += DQ4_WARPS) {
         const int j = x / n, r = x - j * n;
         dq4_put<NG, NT>(p.a + (size_t)j * p.K, (kb0 + 2 * r) * 128, p.K, j, recs + r * C::RECORD);
       }
+      __syncwarp();
       named_bar(1, DQ4_WARPS * 32);
     }
     for (int i = 0; i < nb; i += 2) {

@@ -91,8 +91,10 @@ __device__ __forceinline__ uint4 dt_weights(uint32_t w, uint32_t hi, uint32_t lo
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// (Not the .aligned form: that one needs a warp's lanes to come together, and
+// they come from loops of unequal length.)
 __device__ __forceinline__ void dt_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ float4 dt_ld_cluster4(uint32_t addr, uint32_t rank) {
   float4 v;
@@ -331,6 +333,7 @@ __global__ void __launch_bounds__(DT_THREADS, 1)
   else
     __syncthreads();
   if (warp == DT_WARPS + 1) {
+    __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, p.tmem_cols);
   }
