@@ -130,13 +130,15 @@ __device__ __forceinline__ void dq4_put(const __nv_bfloat16* __restrict__ row, i
   const int k = k0 + 8 * lane;
   const uint4 v = row && k < K ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-  float top = 0.f, s = 0.f;  // the largest finite value; the sum
+  // The largest finite value; the group's sum, of values times 2^-8: as they
+  // come, 32 of 1.1e37 pass the largest f32. (bf16's last place is 2^-133: exact.)
+  float top = 0.f, s = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float x = bf16_lo(w[i]), y = bf16_hi(w[i]);
     if (fabsf(x) < INFINITY) top = fmaxf(top, fabsf(x));
     if (fabsf(y) < INFINITY) top = fmaxf(top, fabsf(y));
-    s += x + y;
+    s = fmaf(x, 0.00390625f, fmaf(y, 0.00390625f, s));
   }
 #pragma unroll
   for (int i = 1; i < 32; i <<= 1) {
@@ -155,7 +157,7 @@ __device__ __forceinline__ void dq4_put(const __nv_bfloat16* __restrict__ row, i
       make_uint4(dq4_pack(bf16_lo(v.x) * f16, bf16_lo(v.z) * f16), dq4_pack(bf16_hi(v.x) * f, bf16_hi(v.z) * f),
                  dq4_pack(bf16_lo(v.y) * f16, bf16_lo(v.w) * f16), dq4_pack(bf16_hi(v.y) * f, bf16_hi(v.w) * f));
   if ((lane & (16 / NG - 1)) == 0)
-    *reinterpret_cast<float*>(blk + 2048 * NT + ((q / (16 / NG)) * 8 * NT + j) * 4) = s * f * -7.62939453125e-06f;
+    *reinterpret_cast<float*>(blk + 2048 * NT + ((q / (16 / NG)) * 8 * NT + j) * 4) = s * f * -0.001953125f;  // 2^8 * -8 * 2^-20
   if (lane == 0)
     *reinterpret_cast<float*>(rec + 2 * dq4_block(NG, NT) + j * 4) = __uint_as_float((uint32_t)(254 - field) << 23);
 }
