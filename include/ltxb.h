@@ -563,9 +563,11 @@ int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k
  * overflow them.) With fewer than 80 query rows a sequence and K/V head
  * (on average: rows * H / kv_heads / batch) the cache is read as it is and its
  * codes enter the products exactly; with more, K and V are laid out in the
- * workspace as f16 (one rounding of 2^-12) for the tcgen05 kernel, which takes
+ * workspace as f16 (one rounding of 2^-12, values down to 2^-29 of the largest
+ * of a sequence and head) for the tcgen05 kernel, which takes
  * 512 bytes per token and head up to the capacity (max_len, if given, is what
- * it is sized by). `workspace` (256-byte aligned,
+ * it is sized by), and weights enter the product as f16 too: with 11 bits down to
+ * 2^-24 of the row's largest, with fewer below, none from 2^-35 on. `workspace` (256-byte aligned,
  * ltxb_attention_kv4_workspace_bytes bytes) need not be cleared; calls that
  * may run at the same time need one each. */
 uint64_t ltxb_attention_kv4_workspace_bytes(const ltxb_kv4_cache* cache, int rows, int H);

@@ -10,8 +10,9 @@
 // warp; S_A S_B | PV_A S_A' | PV_B S_B' | ... with P written over S in TMEM.
 // What differs: a row's own scale (its power of two), a row's own last key
 // (causal, ragged), tiles found from row_start on the device, f16 in place of
-// bf16 for all four operands (P carries 11 bits: the output's own rounding
-// dominates), and NaN scores that must reach the result.
+// bf16 for all four operands (P carries 11 bits down to 2^-24 of a row's
+// largest weight, see kKtLift: the output's own rounding dominates), and NaN
+// scores that must reach the result.
 //
 // Causal tiles are started from the last (longest) to the first, so the short
 // ones fill the end of the grid. With few tiles the keys are split (grid z)
@@ -30,7 +31,15 @@ constexpr int KT_M = 128, KT_N = 128, KT_D = 128, KT_STAGES = 2;
 constexpr int KT_TILE = KT_M * KT_D * 2, KT_HALF = KT_TILE / 2;
 constexpr int KT_THREADS = 576;
 constexpr int KT_SMEM = 1024 + 2 * KT_TILE + 2 * KT_STAGES * KT_TILE + 256 + (2 * 2 * 2 + 2 * 2) * KT_M * 4;
-constexpr float kKtRescale = 8.0f;  // log2 units, as in the bf16 kernel: P stays below 2^8
+// P is 2^10 times p = 2^(score - reference), and a warp's references move when a
+// score of one of its rows passes it by 2^5: P stays below 2^15 in f16, keeps 11
+// bits while p is above 2^-24 and vanishes from 2^-35 on. (As p itself it would
+// vanish from 2^-25 on: 131,072 keys there are 2^-8 of a row's weight, and all of
+// its result if the heaviest key's V is small. The sum l takes the f32 values.)
+// 3,520 x 28,160 tokens, 32 heads: 1,792 us, as without the factor and with moves
+// at 2^8 (1,784); 2^11 and moves at 2^4 take 1,824, and 1,887 where a move is one
+// row's alone: a warp has 32 rows, each of which grows now and then.
+constexpr float kKtRescale = 5.0f, kKtLift = 10.0f, kKtDown = 1.0f / 1024;  // log2 units; 2^-lift
 constexpr uint32_t kKtPoly = 0x2020u;  // pairs of 16 whose exp2 runs as the polynomial (2, as in the bf16 kernel)
 
 struct KtArgs {
@@ -335,7 +344,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
       uint64_t acc2[2];
       uint32_t pk[16];
       auto exp_chunk = [&](const uint32_t* cv) {
-        const uint64_t nm2 = pk2(-m_ref, -m_ref);
+        const uint64_t nm2 = pk2(kKtLift - m_ref, kKtLift - m_ref);
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           float a0, a1, p0, p1;
@@ -366,7 +375,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
       const float cm = sm * cr;
       const bool need = cm > m_ref + kKtRescale;
       if (__any_sync(0xffffffffu, need)) {
-        const float m_new = need ? cm : m_ref;
+        const float m_new = fmaxf(cm, m_ref);  // every row's, once one must (a NaN leaves it)
         const float corr = ex2_mufu(m_ref - m_new);
         m_ref = m_new;
         l *= corr;
@@ -415,10 +424,10 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
       const int tok = row / G, g = row - tok * G;
       const size_t orow = ((size_t)(first + tok) * c.heads + h) * G + g;
       const float gate = (!SPLIT && row_ok && args.gate) ? args.gate[orow] : 1.0f;
-      const float f = SPLIT ? kvs.y : none ? 0.f : gate * kvs.y / lt;
+      const float f = SPLIT ? kvs.y * kKtDown : none ? 0.f : gate * kvs.y / lt;  // (2^10 is in O and in lt)
       const size_t si = state0 + tile * KT_M + r;
       if (SPLIT && row_ok && hf == 0)
-        reinterpret_cast<float2*>(args.t.ml_part)[si] = none ? make_float2(-FLT_MAX, 0.f) : make_float2(m_ref, lt);
+        reinterpret_cast<float2*>(args.t.ml_part)[si] = none ? make_float2(-FLT_MAX, 0.f) : make_float2(m_ref, lt * kKtDown);
 #pragma unroll 1
       for (int cc = 0; cc < 2; ++cc) {
         uint32_t u[32];
