@@ -8,7 +8,7 @@
 //   q . (z + s c)       = s sum q c + z sum q
 //   sum_t p_t (z + s c) = sum (p s) c + sum p z.
 // K: q's values at the first kind of place are held 16 times larger, so that
-// both kinds add up in units of 2^-20. V: the two kinds are rows of their own.
+// both kinds add up in units of 2^-20 (which scores keep, see KA_UNIT). V: the two kinds are rows of their own.
 // (Other forms that were measured at 131,009 tokens x 32 heads: 1 + c / 16 with
 // the offset taken out by one more MMA, 205 us with 16 tokens a step; c - 8 by
 // an f16 FMA a pair, 149; K through the integer MMA with q in two bytes, 136;
@@ -55,6 +55,11 @@
 namespace ltxb {
 
 constexpr int KA_OLD = KV4_D + 4;  // floats per row of the warps' O tiles
+
+// Scores are kept in units of 2^20 up to the exponential: a sum of q times K
+// holds q (at most 2^11 in its row's unit) times 2^-20, so that no K or zero up
+// to bf16's ends overflows it before the row's unit brings it back.
+constexpr float KA_UNIT = 1048576.f, KA_PER = 1.f / KA_UNIT;
 
 struct KaArgs {
   Kv4View c;
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
       for (int e = 0; e < 2; ++e) {
         const int rc = at.rt * R + t * 8 + 2 * cq + e;
         lim[t][e] = a.causal ? at.len - at.count + rc / a.G : at.len - 1;  // last key the row sees
-        m[t][e] = -FLT_MAX;
+        m[t][e] = -FLT_MAX * KA_PER;
       }
       l[t] = 0;
 #pragma unroll
@@ -446,7 +451,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
           const int i = 2 * (x * (8 / NG) + y);
           mma_f16(s, 0x2C002C00u, 0x2C002C00u, 0x3C003C00u, 0x3C003C00u, qf[t][i], qf[t][i + 1]);
         }
-        qs[t][x] = f2(s[0], s[1]);
+        qs[t][x] = f2(KA_PER * s[0], KA_PER * s[1]);
         zs[t][x] = 0;
       }
     }
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
               }
             }
             const uint32_t p0 = kp[x], p1 = kp[8 * NG + x];
-            const float s0 = 1048576.f * bf16_lo(p0), s1 = 1048576.f * bf16_lo(p1), z0 = bf16_hi(p0), z1 = bf16_hi(p1);
+            const float s0 = bf16_lo(p0), s1 = bf16_lo(p1), z0 = bf16_hi(p0), z1 = bf16_hi(p1);  // (codes count 2^-20)
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
               const uint64_t y0 = x ? f2fma(f2(z0, z0), qs[t][x], s[mt][t][0]) : f2mul(f2(z0, z0), qs[t][x]);
@@ -554,7 +559,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
             top[t][0] = mt ? fmax3(top[t][0], x0, x2) : fmaxf(x0, x2);
             top[t][1] = mt ? fmax3(top[t][1], x1, x3) : fmaxf(x1, x3);
           }
-          move = move || top[t][0] > m[t][0] + 8.f || top[t][1] > m[t][1] + 8.f;
+          move = move || top[t][0] > m[t][0] + 8.f * KA_PER || top[t][1] > m[t][1] + 8.f * KA_PER;
         }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
@@ -577,7 +582,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
               float x = fmaxf(m[t][e], top[t][e]);
 #pragma unroll
               for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
-              c[e] = ka_ex2(m[t][e] - x);
+              c[e] = ka_ex2((m[t][e] - x) * KA_UNIT);
               m[t][e] = x;
               f[e] = c[e] * turn;
             }
@@ -597,11 +602,11 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
           uint64_t p2[NT][2];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const uint64_t nm = f2(-m[t][0], -m[t][1]);
+            const uint64_t nm = f2(-KA_UNIT * m[t][0], -KA_UNIT * m[t][1]), un = f2(KA_UNIT, KA_UNIT);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               float x0, x1;
-              un2(f2add(s[mt][t][y], nm), x0, x1);
+              un2(f2fma(s[mt][t][y], un, nm), x0, x1);
               p2[t][y] = f2(ka_ex2(x0), ka_ex2(x1));
               l[t] = f2add(l[t], p2[t][y]);
             }
@@ -670,7 +675,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
           for (int x = 0; x < NG; ++x) lt[e] += (z[x][e] - z[x][e]) + (o[t][8 / NG * x][e] - o[t][8 / NG * x][e]);
           const int r = t * 8 + 2 * cq + e;
           if (g == 0) {
-            sm.m[warp][r] = m[t][e];
+            sm.m[warp][r] = KA_UNIT * m[t][e];
             sm.l[warp][r] = lt[e];
           }
 #pragma unroll

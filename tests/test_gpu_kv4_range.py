@@ -15,7 +15,7 @@ import pytest
 import torch
 
 from oracle import kv4_ref as kr
-from test_gpu_kv4 import make_cache
+from test_gpu_kv4 import check, check_many, make_cache
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,41 @@ def test_many_rows_under_one_heavy_token(cuda, nats, T, at, rows, causal, group)
     out = ltxb.attention_kv4(q, cache, causal=causal, scale=1.0)
     agrees(out, q, kr.held(k.cpu(), group), kr.held(v.cpu(), group), causal)
     assert ltxb.device_status() == ltxb.OK
+
+
+UNEQUAL = [(1e-30, 1e30, 1e-30), (1e25, 1e-25, 1e30), (1.0, 1.0, 1e-37), (1e-38, 1e-5, 1.0), (1e-33, 1e33, 1.0),
+           (1e-37, 2e37, 1e-20), (1e36, 1e-36, 1.0), (1e37, 1e-37, 1e28)]
+
+
+@pytest.mark.parametrize("qs,ks,vs", UNEQUAL)
+@pytest.mark.parametrize("rows,group", [(1, 128), (8, 64), (10, 32), (16, 64)])
+def test_few_rows_of_unequal_size(cuda, rows, group, qs, ks, vs):
+    """Queries, keys and values over many powers of two, up to bf16's ends."""
+    import ltxb
+    T, H = 200, 2
+    g = torch.Generator().manual_seed(3)
+    q = (torch.randn(rows, H, 128, generator=g) * qs * torch.exp2(torch.arange(rows) % 5 - 2.0)[:, None, None])
+    k, v = (torch.randn(T, H, 128, generator=g) * s for s in (ks, vs))
+    q, k, v = q.to(torch.bfloat16), k.to(torch.bfloat16), v.to(torch.bfloat16)
+    cache = make_cache([T], H, group, cuda)
+    cache.append(k.to(cuda), v.to(cuda))
+    out = ltxb.attention_kv4(q.to(cuda), cache)
+    kh, vh = kr.held(k, group), kr.held(v, group)
+    check(out, kr.attention(q, kh, vh, True), float(vh.abs().max()))
+    assert ltxb.device_status() == ltxb.OK
+
+
+@pytest.mark.parametrize("qs,ks", [(1e-33, 1e33), (1e-37, 2e37), (1e36, 1e-36)])
+def test_many_rows_of_unequal_size_too(cuda, qs, ks):
+    """The same sizes give the same answer on both sides of the number of rows that chooses the kernel."""
+    import ltxb
+    T, H = 200, 2
+    g = torch.Generator().manual_seed(3)
+    q = (torch.randn(100, H, 128, generator=g) * qs).to(torch.bfloat16)
+    k, v = (torch.randn(T, H, 128, generator=g) * ks).to(torch.bfloat16), torch.randn(T, H, 128, generator=g).to(torch.bfloat16)
+    cache = make_cache([T], H, 64, cuda)
+    cache.append(k.to(cuda), v.to(cuda))
+    kh, vh = kr.held(k, 64), kr.held(v, 64)
+    check_many(ltxb.attention_kv4(q.to(cuda), cache), kr.attention(q, kh, vh, True), q, kh, vh)
+    few = q[-16:]
+    check(ltxb.attention_kv4(few.to(cuda), cache), kr.attention(few, kh, vh, True), float(vh.abs().max()))
