@@ -562,7 +562,8 @@ int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k
  * accumulators are f32. (Sums hold p up to 2^8 times V: |V| below 2^100 cannot
  * overflow them.) With fewer than 80 query rows a sequence and K/V head
  * (on average: rows * H / kv_heads / batch) the cache is read as it is and its
- * codes enter the products exactly; with more, K and V are laid out in the
+ * codes enter the products exactly, a weight times a token's scale as f16 (11
+ * bits down to 2^-23 of the row's largest such product); with more, K and V are laid out in the
  * workspace as f16 (one rounding of 2^-12, values down to 2^-29 of the largest
  * of a sequence and head) for the tcgen05 kernel, which takes
  * 512 bytes per token and head up to the capacity (max_len, if given, is what

@@ -20,10 +20,12 @@
 // the same as one: S^T = K Q^T, then O^T = V^T P^T with P^T transposed in
 // registers (movmatrix). q enters as f16 after a power of two per row (its 8
 // bits stay exact down to 2^-27 of the row's largest value). p s enters as f16
-// scaled by a power of two that follows the largest V scale seen (between 2^3
-// and 2^7 times p): 11 significant bits where bf16 would keep 8, so the
-// result's own rounding dominates. Row maxima move only when a score passes
-// them by 2^8; sums and accumulators are f32.
+// after a power of two per row, which keeps the largest p s that the row has met
+// between 2^9 and 2^15: 11 significant bits down to 2^-23 of that, where bf16
+// would keep 8, so the result's own rounding dominates, and nothing from 2^-34
+// on. It goes by p s, not by p or s: neither a heavy token of small V nor a large
+// V without weight pushes the others out. Row maxima (whole numbers) move only
+// when a score passes them by 2^8, or with the powers; sums and accumulators are f32.
 //
 // Work is split by pages, not by sequence: all (sequence, head, row tile)
 // items laid end to end are one line of pages (each item with KA_ITEM more,
@@ -60,6 +62,13 @@ constexpr int KA_OLD = KV4_D + 4;  // floats per row of the warps' O tiles
 // holds q (at most 2^11 in its row's unit) times 2^-20, so that no K or zero up
 // to bf16's ends overflows it before the row's unit brings it back.
 constexpr float KA_UNIT = 1048576.f, KA_PER = 1.f / KA_UNIT;
+// The largest power of two that p takes on its way to f16 (p is at most 2^8:
+// the product stays a number) and its exponent's field; where it starts.
+constexpr float KA_SG_MAX = 6.646139978924579e35f;  // 2^119
+constexpr int KA_SG_FIELD = 127 + 119;
+// Where the largest p s of a row goes when it moves: 64 sequences of 17 to 8,192
+// tokens took 107 us with 8 and 9, 121 with 11 (a move looked at every group's scale then; 92 now).
+constexpr int KA_SG_TO = 9;
 
 struct KaArgs {
   Kv4View c;
@@ -457,7 +466,9 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
     }
     // keys that every row of the tile sees: up to the first row's
     const int all = a.causal ? at.len - at.count + (at.rt * R) / a.G : at.len - 1;
-    float sig = 1.f, sig_max = 0.f;  // p s is held as p * (s * sig); sig moves when s passes sig_max
+    uint64_t sg[NT];  // rows 2 c, 2 c + 1: p s enters the product as p * sg * s
+#pragma unroll
+    for (int t = 0; t < NT; ++t) sg[t] = f2(KA_SG_MAX, KA_SG_MAX);
     const int npg = at.pb - at.pa > warp ? (at.pb - at.pa - warp + NW - 1) / NW : 0;
     for (int k = 0; k < npg; ++k, ++used) {
       if (ok) ok = warp_wait(&sm.kfull[warp], used & 1, 0x301);
@@ -546,8 +557,10 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
               }
             }
         }
-        // ---- reference maxima and the V power move only when they must ----
-        bool move = svm > sig_max;
+        // ---- reference maxima and the powers of p s move only when they must, all rows' then: when a score
+        // passes its maximum by 2^8, or some p sg s may pass 2^15 (the lane's largest p times its largest
+        // scale, which need not be one token's) ----
+        bool move = false;
         float top[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -559,33 +572,56 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
             top[t][0] = mt ? fmax3(top[t][0], x0, x2) : fmaxf(x0, x2);
             top[t][1] = mt ? fmax3(top[t][1], x1, x3) : fmaxf(x1, x3);
           }
-          move = move || top[t][0] > m[t][0] + 8.f * KA_PER || top[t][1] > m[t][1] + 8.f * KA_PER;
+          float g0, g1;
+          un2(sg[t], g0, g1);
+          const float d0 = (top[t][0] - m[t][0]) * KA_UNIT, d1 = (top[t][1] - m[t][1]) * KA_UNIT;
+          move = move || d0 > 8.f || d1 > 8.f || ka_ex2(d0) * g0 * svm > 32768.f || ka_ex2(d1) * g1 * svm > 32768.f;
         }
         if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
-          for (int i = 4; i < 32; i <<= 1) svm = fmaxf(svm, __shfl_xor_sync(0xffffffffu, svm, i));
-          float turn = 1.f;
-          if (svm > sig_max) {  // the same in every lane
-            // sig = 2^(3 - floor(log2 svm)): s * sig in [8, 16) now, at most 128 before it moves again
-            int ex = 257 - (int)(__float_as_uint(svm) >> 23);
-            ex = ex > 253 ? 253 : ex < 1 ? 1 : ex;
-            const float ns = __uint_as_float((uint32_t)ex << 23);
-            turn = ns / sig;
-            sig = ns;
-            sig_max = 128.f / ns;
-          }
-#pragma unroll
           for (int t = 0; t < NT; ++t) {
-            float c[2], f[2];
+            float c[2], f[2], g2[2], most[2] = {0.f, 0.f};  // most: each row's largest p s, times 2^-20
+            int was[2];
+            un2(sg[t], g2[0], g2[1]);
+            // maxima to the next whole number: sg can grow by the power of two that p loses
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(m[t][e], top[t][e]);
+              float x = top[t][e];
 #pragma unroll
               for (int i = 4; i < 32; i <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, i));
-              c[e] = ka_ex2((m[t][e] - x) * KA_UNIT);
+              x = fmaxf(m[t][e], ceilf(x * KA_UNIT) * KA_PER);
+              const float d = (x - m[t][e]) * KA_UNIT;
+              c[e] = ka_ex2(-d);
               m[t][e] = x;
-              f[e] = c[e] * turn;
+              was[e] = (int)(__float_as_uint(g2[e]) >> 23) + (int)fminf(d, 512.f);  // field of the sg that leaves O as it is
             }
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                // the token's largest scale (a NaN drops out of the maximum below, as does whatever a p of 0 stands before)
+                uint32_t w = 0;
+                float x0, x1;
+#pragma unroll
+                for (int x = 0; x < NG; ++x) w = __vmaxu2(w, vp[(mt * 16 + y * 8) * NG + x]);
+                const float sc = KA_PER * bf16_lo(w);
+                un2(s[mt][t][y], x0, x1);
+                most[0] = fmaxf(most[0], sc * ka_ex2((x0 - m[t][0]) * KA_UNIT));
+                most[1] = fmaxf(most[1], sc * ka_ex2((x1 - m[t][1]) * KA_UNIT));
+              }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+              for (int i = 4; i < 32; i <<= 1) most[e] = fmaxf(most[e], __shfl_xor_sync(0xffffffffu, most[e], i));
+              // fields: with sg's at f, p s sg lies in [2^(to + f - 254 + 20), twice that); in [2^KA_SG_TO, twice that) at most from now on
+              const int to = (int)(__float_as_uint(most[e]) >> 23);
+              int now = was[e] < KA_SG_FIELD ? was[e] : KA_SG_FIELD;
+              if (to > 0 && now > 254 - 20 + KA_SG_TO - to) now = 254 - 20 + KA_SG_TO - to;
+              now = now < 1 ? 1 : now;
+              g2[e] = __uint_as_float((uint32_t)now << 23);
+              f[e] = was[e] - now < 127 ? __uint_as_float((uint32_t)(127 - (was[e] - now)) << 23) : 0.f;
+            }
+            sg[t] = f2(g2[0], g2[1]);
             l[t] = f2mul(l[t], f2(c[0], c[1]));
 #pragma unroll
             for (int x = 0; x < NG; ++x) zs[t][x] = f2mul(zs[t][x], f2(c[0], c[1]));
@@ -599,7 +635,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
           uint32_t pb[NT][NG][2];
-          uint64_t p2[NT][2];
+          uint64_t p2[NT][2], pg[NT][2];
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             const uint64_t nm = f2(-KA_UNIT * m[t][0], -KA_UNIT * m[t][1]), un = f2(KA_UNIT, KA_UNIT);
@@ -609,6 +645,7 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
               un2(f2fma(s[mt][t][y], un, nm), x0, x1);
               p2[t][y] = f2(ka_ex2(x0), ka_ex2(x1));
               l[t] = f2add(l[t], p2[t][y]);
+              pg[t][y] = f2mul(p2[t][y], sg[t]);
             }
           }
 #pragma unroll
@@ -621,12 +658,11 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
                 const int key = page0 + (h * MT + mt) * 16 + y * 8 + g;
                 if (key >= at.len || !good || !(fabsf(sc + zv) < INFINITY)) sc = zv = 0.f;
               }
-              const float f = sc * sig;
 #pragma unroll
               for (int t = 0; t < NT; ++t) {
                 zs[t][x] = f2fma(p2[t][y], f2(zv, zv), zs[t][x]);
                 float x0, x1;
-                un2(f2mul(p2[t][y], f2(f, f)), x0, x1);
+                un2(f2mul(pg[t][y], f2(sc, sc)), x0, x1);
                 pb[t][x][y] = transpose8x8(pack_f16x2(x0, x1));
               }
             }
@@ -655,11 +691,13 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
     }
     // ---- the item, or this CTA's piece of it, is done: join the warps ----
     if (ok) {
-      const float back0 = 16777216.f / sig, back1 = 1048576.f / sig;  // 2^24, 2^20
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        float lt[2], z[NG][2];
+        float lt[2], z[NG][2], back[2];
         un2(l[t], lt[0], lt[1]);
+        un2(sg[t], back[0], back[1]);  // powers of two: 1 / sg from the exponent's field
+        back[0] = __uint_as_float((254u << 23) - __float_as_uint(back[0]));
+        back[1] = __uint_as_float((254u << 23) - __float_as_uint(back[1]));
 #pragma unroll
         for (int x = 0; x < NG; ++x) un2(zs[t][x], z[x][0], z[x][1]);
 #pragma unroll
@@ -682,8 +720,9 @@ __global__ void __launch_bounds__(KA_THREADS, KA_PER_SM) kv4_attn_kernel(const K
           for (int j = 0; j < 4; ++j) {
             const float zz = z[j * NG / 4][e];
             *reinterpret_cast<float4*>(&sm.o[warp][r][32 * j + 4 * g]) =
-                make_float4(fmaf(o[t][2 * j][e], back0, zz), fmaf(o[t][2 * j][2 + e], back1, zz),
-                            fmaf(o[t][2 * j + 1][e], back0, zz), fmaf(o[t][2 * j + 1][2 + e], back1, zz));
+                make_float4(fmaf(16777216.f * o[t][2 * j][e], back[e], zz), fmaf(1048576.f * o[t][2 * j][2 + e], back[e], zz),
+                            fmaf(16777216.f * o[t][2 * j + 1][e], back[e], zz),
+                            fmaf(1048576.f * o[t][2 * j + 1][2 + e], back[e], zz));  // codes count 2^-24 and 2^-20
           }
         }
       }
