@@ -490,8 +490,8 @@ int ltxb_stats(const float* v, uint64_t n, float* out, void* workspace, uint64_t
  *
  * Values: the 128 values of a token's head fall into groups of `group` = 32,
  * 64 or 128; each group stores zero = min and scale = bf16((max - min) / 15)
- * as bf16, and per value code = round((x - zero) / scale) in 0 .. 15 (the
- * differences in f32, the quotients exact, ties to even, 0 where scale is 0).
+ * as bf16, and per value code = round((x - zero) / scale) in 0 .. 15 (all of it
+ * exact, ties to even, 0 where scale is 0).
  * A code stands for zero + scale * code. A group that holds a NaN or an
  * infinity, or whose range is above the largest f32, reads back as NaN.
  *

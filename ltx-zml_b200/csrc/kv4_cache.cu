@@ -3,12 +3,22 @@
 //
 // Quantiser, per token, head and group of 32 / 64 / 128 values x (bf16):
 //   zero = min x, scale = bf16((max x - min x) / 15), code = round((x - zero) / scale),
-// the differences in f32, the quotients exact, ties to even, code 0 where scale
-// is 0. A quotient is a product with 1 / scale and one Newton step: exact where
-// it is a half (ties are common, both sides having few bits) and within 5e-7
-// elsewhere, where no quotient of an f32 difference below 15.06 scales by an
-// 8-bit scale comes closer to a half than 9e-7. scale is at least
-// range / 15 * (1 - 2^-8), so the quotient stays below 15.06: no clamp.
+// all of it exact, ties to even, code 0 where scale is 0. A quotient is a product
+// with 1 / scale and one Newton step: off by at most 0.5001 units of its last
+// place, and a half where it is one (ties are common, both sides having few bits).
+// Elsewhere the quotient of an f32 difference d by the 8-bit scale s stays 0.5019
+// units away from each half h (h s is an f32 number, so d is a unit or more from
+// it: 2^-23 / m(h s) of it, m the mantissa in [1, 2), at most 2 - 2^-7, where half
+// a unit of h is 2^-24 / m(h)): it falls on its own side. A difference is an f32
+// number unless a value's exponent lies 16 or more below another's; rounding
+// it can then only make a tie, never pass one, and what was rounded off decides
+// that tie. Such a tie is the larger of the two itself, for it has 8 bits and h s
+// has 13, and the smaller is 2^-24 of it or less: zero = -h s, with some x close to
+// 0, or x = h s and zero close to 0. A token's K or V whose zero is the one or the
+// other is done again with care. (That takes 8 us of the time below;
+// looking at all values for small ones 11 to 30.) scale is at least range / 15 * (1 - 2^-8), so the
+// quotient stays below 15.06: no clamp. (scale itself needs no such care: 15 times a
+// bf16 midpoint has more than 8 bits and is no sum of one value and a far smaller one.)
 // A group that holds a NaN or an infinity (or whose range is above the
 // largest f32) stores scale = NaN and reads back as NaN.
 //
@@ -99,9 +109,24 @@ __device__ __forceinline__ uint64_t c2fma(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
+// Code c of x - zero: where its f32 value over scale is a tie, what was rounded off decides.
+__device__ __forceinline__ float kv4_settle(float c, float x, float zero, float scale) {
+  const float d = x - zero, b = d - x, off = (x - (d - b)) + (-zero - b);  // x - zero = d + off
+  const float rest = fmaf(-scale, c, d), half = 0.5f * scale;
+  return rest == half && off > 0.f ? c + 1.f : rest == -half && off < 0.f ? c - 1.f : c;
+}
+
+// Whether a group of this pair may hold such ties (a pair of NaN does not).
+__device__ __forceinline__ bool kv4_unsettled(uint32_t pair) {
+  const float scale = bf16_lo(pair), zero = bf16_hi(pair);
+  const float q = __fdiv_rn(-zero, scale);
+  return fabsf(q - rintf(q)) == 0.5f || (zero != 0.f && fabsf(zero) * 8388608.f <= 16.f * scale);
+}
+
 // Eight codes (nibble i = value i of a lane's eight consecutive dims) and the
-// group's (scale, zero) pair; the 16 / NG lanes of a group agree.
-template <int NG>
+// group's (scale, zero) pair; the 16 / NG lanes of a group agree. Without SETTLE
+// ties that only rounding made are as they fall.
+template <int NG, bool SETTLE>
 __device__ __forceinline__ uint32_t kv4_quantise(uint4 v, uint32_t* pair) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   // (max, -min) as one bf16x2: one shuffle and one maximum per step
@@ -130,6 +155,13 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint4 v, uint32_t* pair) {
     const uint64_t t1 = c2fma(c2fma(ns, t, d), in2, t);
     c2un(c2add(c2add(t1, mg), nm), q[2 * i], q[2 * i + 1]);  // the nearest integers (1.5 * 2^23 added and taken off)
   }
+  if (SETTLE) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      q[2 * i] = kv4_settle(q[2 * i], bf16_lo(w[i]), zero, scale);
+      q[2 * i + 1] = kv4_settle(q[2 * i + 1], bf16_hi(w[i]), zero, scale);
+    }
+  }
   uint32_t code[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {  // four codes as one exact number below 2^16, in the low bits of 1.5 * 2^23
@@ -143,7 +175,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(uint4 v, uint32_t* pair) {
 #pragma unroll 1
       for (int i = 0; i < 8; ++i) {
         const float x = __uint_as_float(i & 1 ? w[i >> 1] & 0xFFFF0000u : w[i >> 1] << 16);
-        out |= (uint32_t)fminf(rintf(__fdiv_rn(x - zero, scale)), 15.f) << (4 * i);
+        out |= (uint32_t)kv4_settle(fminf(rintf(__fdiv_rn(x - zero, scale)), 15.f), x, zero, scale) << (4 * i);
       }
   }
   return out;
@@ -156,6 +188,7 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const Kv4View c, con
                                                          size_t ldk, const __nv_bfloat16* __restrict__ v,
                                                          size_t ldv) {
   __shared__ __align__(16) uint8_t codes[8][2][512];
+  __shared__ uint32_t pairs[8][4][2][2 * NG];
   const int warp = warp_id(), lane = lane_id(), half = lane >> 4, m = lane & 15;
   const int h = blockIdx.y * 8 + warp;
   if (h >= c.heads) return;
@@ -175,21 +208,46 @@ __global__ void __launch_bounds__(256, 4) kv4_append_kernel(const Kv4View c, con
   if (page < 0) return;
   uint8_t* blk = const_cast<uint8_t*>(kv4_block_at(c, page, h, kv4_block(NG)));
   const int j = m >> 2, cc = m & 3;  // dims 32 j + 8 cc .. + 7
+  auto put_k = [&](int t, uint32_t kc) { *reinterpret_cast<uint32_t*>(&codes[warp][0][t * 64 + (cc * 4 + j) * 4]) = kc; };
+  auto put_v = [&](int t, uint32_t vc) {  // halves j of chunks 2 cc and 2 cc + 1
+    uint8_t* vd = &codes[warp][1][2 * cc * 64 + (t >> 1) * 16 + (t & 1) * 8 + j * 2];
+    *reinterpret_cast<uint16_t*>(vd) = (uint16_t)vc;
+    *reinterpret_cast<uint16_t*>(vd + 64) = (uint16_t)(vc >> 16);
+  };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int t = 2 * i + half, pos = base + t;
     uint32_t kp, vp;
-    const uint32_t kc = kv4_quantise<NG>(x[0][i], &kp), vc = kv4_quantise<NG>(x[1][i], &vp);
-    *reinterpret_cast<uint32_t*>(&codes[warp][0][t * 64 + (cc * 4 + j) * 4]) = kc;
-    // halves j of chunks 2 cc and 2 cc + 1
-    uint8_t* vd = &codes[warp][1][2 * cc * 64 + (t >> 1) * 16 + (t & 1) * 8 + j * 2];
-    *reinterpret_cast<uint16_t*>(vd) = (uint16_t)vc;
-    *reinterpret_cast<uint16_t*>(vd + 64) = (uint16_t)(vc >> 16);
-    if (m % (16 / NG) == 0 && pos >= oc.p0 && pos < oc.p1) {
-      const int at = ((t8 * 8 + t) * NG + m / (16 / NG)) * 4;
-      *reinterpret_cast<uint32_t*>(blk + KV4_KPAIR + at) = kp;
-      *reinterpret_cast<uint32_t*>(blk + kv4_vpair(NG) + at) = vp;
+    put_k(t, kv4_quantise<NG, false>(x[0][i], &kp));
+    put_v(t, kv4_quantise<NG, false>(x[1][i], &vp));
+    if (m % (16 / NG) == 0) {
+      pairs[warp][i][0][lane / (16 / NG)] = kp;
+      pairs[warp][i][1][lane / (16 / NG)] = vp;
+      if (pos >= oc.p0 && pos < oc.p1) {
+        const int at = ((t8 * 8 + t) * NG + m / (16 / NG)) * 4;
+        *reinterpret_cast<uint32_t*>(blk + KV4_KPAIR + at) = kp;
+        *reinterpret_cast<uint32_t*>(blk + kv4_vpair(NG) + at) = vp;
+      }
     }
+  }
+  __syncwarp();
+  // the calls (token pair, K or V) whose groups may hold unsettled ties: a pair or two a lane
+  uint32_t again = 0;
+#pragma unroll
+  for (int u = lane; u < 16 * NG; u += 32)
+    if (kv4_unsettled((&pairs[warp][0][0][0])[u])) again |= 1u << (u / (2 * NG));
+  again = __reduce_or_sync(0xffffffffu, again);
+#pragma unroll 1
+  for (; again; again &= again - 1) {
+    const int n = __ffs(again) - 1, t = 2 * (n >> 1) + half, pos = base + t;
+    const size_t row = pos >= oc.p0 && pos < oc.p1 ? oc.row0 + (pos - oc.p0) : oc.row0;
+    uint32_t pair;
+    const uint32_t code = kv4_quantise<NG, true>(
+        __ldg(reinterpret_cast<const uint4*>((n & 1 ? v + row * ldv : k + row * ldk) + h * KV4_D + 8 * m)), &pair);
+    if (n & 1)
+      put_v(t, code);
+    else
+      put_k(t, code);
   }
   __syncwarp();
   const uint4 ko = *reinterpret_cast<const uint4*>(&codes[warp][0][lane * 16]);

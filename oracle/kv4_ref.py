@@ -24,12 +24,17 @@ def quantise(x: torch.Tensor, group: int):
     """codes [..., 128] int64, scale and zero [..., 128 / group] float64 of bf16-valued x [..., 128]."""
     g = x.double().reshape(*x.shape[:-1], HD // group, group)
     zero = g.amin(-1)
-    rng = (g.amax(-1) - zero).float().double()  # the format's differences are those of f32
+    rng = g.amax(-1) - zero
     scale = bf16(rng / 15)
-    d = (g - zero[..., None]).float().double()
-    q = torch.where(scale[..., None] > 0, d / scale[..., None], torch.zeros_like(g))
+    s, z = scale[..., None], zero[..., None]
+    d = g - z
+    b = d - g
+    off = (g - (d - b)) + (-z - b)  # g - z = d + off: a difference beyond 53 bits leaves a remainder,
+    q = torch.where(s > 0, d / s, torch.zeros_like(g))
     code = torch.round(q).clamp(0, 15)
-    bad = ~torch.isfinite(rng)
+    rest = d - s * code             # which decides what only rounding made a tie
+    code = code + ((s > 0) & (rest == s / 2) & (off > 0)) - (1.0 * ((s > 0) & (rest == -s / 2) & (off < 0)))
+    bad = ~torch.isfinite(rng.float())
     scale = torch.where(bad, torch.full_like(scale, math.nan), scale)
     code = torch.where(bad[..., None], torch.zeros_like(code), code)
     return code.to(torch.int64).reshape(x.shape), scale, zero
