@@ -15,8 +15,8 @@
 // that tie. Such a tie is the larger of the two itself, for it has 8 bits and h s
 // has 13, and the smaller is 2^-24 of it or less: zero = -h s, with some x close to
 // 0, or x = h s and zero close to 0. A token's K or V whose zero is the one or the
-// other is done again with care. (That takes 8 us of the time below;
-// looking at all values for small ones 11 to 30.) scale is at least range / 15 * (1 - 2^-8), so the
+// other is done again with care (8 us of the time below; looking at all values
+// for small ones took 11 to 30). scale is at least range / 15 * (1 - 2^-8), so the
 // quotient stays below 15.06: no clamp. (scale itself needs no such care: 15 times a
 // bf16 midpoint has more than 8 bits and is no sum of one value and a far smaller one.)
 // A group that holds a NaN or an infinity (or whose range is above the

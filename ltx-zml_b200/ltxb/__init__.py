@@ -882,6 +882,7 @@ def attention_split(q, k, v, gate=None, splits: int = 0, scale: float | None = N
 # ---------------------------------------------------------------------------
 
 KV4_PAGE = 64
+_NEED_MAX = 64
 SITE_KV4_PAGE, SITE_KV4_LEN, SITE_KV4_ROWS = 0x401, 0x402, 0x403
 
 
@@ -955,7 +956,7 @@ class KV4Cache:
         self._c = _KV4(pages.data_ptr(), None if page_table is None else page_table.data_ptr(), seq_lens.data_ptr(),
                        pages.shape[0], self.kv_heads, group, self.batch, max_pages, int(max_len))
         self._ref = ctypes.byref(self._c)
-        self._need = {}  # workspace bytes of attention calls by (rows, H)
+        self._need = {}  # workspace bytes of attention calls by (rows, H), of _NEED_MAX sizes at most
 
     @property
     def pages(self):
@@ -1037,6 +1038,8 @@ def attention_kv4(q, cache: KV4Cache, row_start=None, causal: bool = True, gate=
     if workspace is None:
         need = cache._need.get((rows, H))
         if need is None:
+            if len(cache._need) >= _NEED_MAX:  # calls of ever other sizes
+                cache._need.clear()
             with _device(cache.device):  # its size goes by the device's number of SMs
                 need = cache._need[rows, H] = lib.ltxb_attention_kv4_workspace_bytes(cache._ref, rows, H)
         workspace = _scratch(need, cache.device, stream)
