@@ -365,6 +365,7 @@ __global__ void __launch_bounds__(KT_THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ch == 0 ? &p_half[tile] : &p_full[tile]);
+        __syncwarp();  // (the next TMEM access takes the whole warp)
       };
       acc2[0] = acc2[1] = pk2(0.f, 0.f);
       exp_chunk(c0);  // with the current reference; redone below if that moves
