@@ -557,10 +557,10 @@ int ltxb_kv4_read(const ltxb_kv4_cache* cache, const int32_t* row_start, void* k
  * [rows, H, 128] bf16 (q's row stride ldq elements; out contiguous), query
  * head h reading K/V head h / (H / kv_heads). causal != 0: a row sees the
  * tokens up to its own; else all of its sequence's. A row that sees nothing
- * is zero; a row of q that is not finite is NaN. `gate` (optional, f32 [rows, H]) multiplies each head's output.
- * A row that attends to a token with a NaN group is NaN. Softmax, sums and
- * accumulators are f32. (Sums hold p up to 2^8 times V: |V| below 2^100 cannot
- * overflow them.) With fewer than 80 query rows a sequence and K/V head
+ * is zero; any other row of q that is not finite is NaN. `gate` (optional, f32
+ * [rows, H]) multiplies each head's output. A row that attends to a token with a
+ * NaN group is NaN. Softmax, sums and accumulators are f32. (Sums hold p up to 2^8
+ * times V: |V| below 2^100 cannot overflow them.) With fewer than 80 query rows a sequence and K/V head
  * (on average: rows * H / kv_heads / batch) the cache is read as it is and its
  * codes enter the products exactly, a weight times a token's scale as f16 (11
  * bits down to 2^-23 of the row's largest such product); with more, K and V are laid out in the
@@ -585,7 +585,7 @@ int ltxb_attention_kv4(const ltxb_kv4_cache* cache, const int32_t* row_start, co
  * weights as they are, with exact products and f32 sums (the workspace holds A
  * in the order of the matrix fragments; a row of A that is not finite gives
  * NaN). More rows round them once to bf16, on their way to the tensor cores, or
- * above 1,024 rows in `workspace` (N * K * 2 bytes). Each call writes what it
+ * above 1,024 rows in `workspace` (N * K * 2 bytes); an infinity in A can stay one there. Each call writes what it
  * reads of the workspace (ltxb_dq4_gemm_workspace_bytes bytes on the current
  * device, 0 where none is needed); calls that may run at the same time need one
  * each. */

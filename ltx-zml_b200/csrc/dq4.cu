@@ -27,8 +27,8 @@
 // TB/s); 8 x 36,864 x 4,096, groups of 128: 24 us; 16 x 4,096 x 16,384, groups
 // of 32: 28 us; 16 x 16,384 x 4,096: 22 us. What bounds it there is the start
 // (A's records, first tiles: 3.5 us), the instructions of a tile (the scale
-// and start value of every group and output) and the cluster's sum (3 us), no
-// longer the bytes. (Four warps of 32 rows each: 27, 27, 42 and 21 us.)
+// and start value of every group and output) and their latencies, and where K is
+// split (not with 36,864 rows) the cluster's sum (3 us), no longer the bytes. (Four warps of 32 rows each: 27, 27, 42 and 21 us.)
 //
 // 17 to 1,024 rows (DQ4_TC_ROWS): the tcgen05 kernel of dq4_tc.cu, which makes
 // bf16 weights (one rounding: the code and a bf16 scale have up to 11

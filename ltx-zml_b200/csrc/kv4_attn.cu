@@ -38,12 +38,13 @@
 // arrives while it works on V, the next V while it works on K, and no barrier
 // joins the warps until an item ends.
 //
-// Measured: 131,009 tokens x 32 heads, groups of 128 (570 MB): 117 us, 4.9 TB/s;
-// the loads alone take 95. 64 sequences of 17 to 8,192 tokens, 32 heads over 8,
-// groups of 32 (328 MB): 93 us. 8 of 900 to 2,500, 16 rows each: 26 us. What bounds it is the instructions of a tile
-// (230 per 16 tokens, the ALU pipe 59 % busy) under 12 warps an SM; two buffers
-// each for K and V, or 16 warps, gained nothing. One sequence of 77 tokens: 12
-// us for both kernels, latencies from the lengths to the join.
+// Measured: 131,009 tokens x 32 heads, groups of 128 (570 MB): 113 to 121 us, 4.9
+// TB/s; the loads alone take 95. 64 sequences of 17 to 8,192 tokens, 32 heads over
+// 8, groups of 32 (328 MB): 92 us. 8 of 900 to 2,500, 16 rows each: 24 us from L2,
+// 31 without. What bounds it is the instructions of a tile (230 per 16 tokens, the
+// ALU pipe 59 % busy) under 12 warps an SM; two buffers each for K and V, or 16
+// warps, gained nothing. One sequence of 77 tokens: 12 us for both kernels,
+// latencies from the lengths to the join.
 //
 // A token whose V group is stored as NaN, or whose page number is bad, makes
 // every row that attends to it NaN and no others: where a page holds tokens
@@ -939,8 +940,8 @@ static int ka_launch(const KaArgs& a, int ctas, cudaStream_t st) {
   if (e != cudaSuccess) return set_cuda_error(e, "kv4 attention launch");
   cudaLaunchConfig_t cfg{};
   // Items of few pieces (on average): a row a warp, and an eighth of the CTAs, most of
-  // which find nothing to join. 8 x 1,700 tokens x 8 heads, 16 rows: 32 us instead of
-  // 36; 4 x 4,000, 64 rows: 52 and 60. With 14 pieces an item (131,009 tokens x 32
+  // which find nothing to join. 8 x 1,700 tokens x 8 heads, 16 rows, without L2: 32 us
+  // instead of 36; 4 x 4,000, 64 rows: 52 and 60. With 14 pieces an item (131,009 tokens x 32
   // heads) 124 and 122.
   const int64_t tiles = (int64_t)a.c.rows * a.G / R;
   const bool warp_rows = ctas <= KA_FEW * (tiles > a.c.batch ? tiles : a.c.batch) * a.c.heads;
